@@ -36,6 +36,11 @@ extern "C" {
 #define NERF_E_LAUNCH (-2)  /* HIP reported an error at launch */
 #define NERF_E_ARCH (-3)    /* the current device is not gfx950 */
 
+/* element types of the entry points that take more than fp32 */
+#define NERF_F32 0
+#define NERF_BF16 1
+#define NERF_F16 2
+
 /* ---- probes ------------------------------------------------------------------------------- */
 int nerf_version(void);                 /* ABI version, currently 1 */
 const char* nerf_arch(void);            /* "gfx950": the only code object in the library */
@@ -375,6 +380,66 @@ int nerf_linear_bwd_data(int64_t n, int n_in, int n_out, const float* dy, int64_
 int64_t nerf_linear_workspace_floats(int n_in, int n_out);
 int nerf_linear_bwd_weights(int64_t n, int n_in, int n_out, const float* dy, int64_t ldy, const float* x, int64_t ldx, float* dw,
                             float* db, float* workspace, void* stream);
+
+/* ---- layers and optimiser of networks the fused kernels do not cover --------------------------------------------------
+ * Layer norm over the last dimension (no counterpart upstream; NeRF(layer_norm=True) calls it).  x, y, dy, dx: [n, c] of `type`
+ * (NERF_F32 / NERF_BF16 / NERF_F16) with row strides ld* in elements; w, b: [c] of w_type (`type` or NERF_F32), either may be
+ * NULL (ones, zeros).  1 <= c <= NERF_LAYER_NORM_MAX_C.  Sums and statistics in fp32, each output rounded once.
+ * nerf_layer_norm_fwd: y = (x - mean) / sqrt(var + eps) * w + b.  stats: NULL, or 3 n floats for the backward pass (the mean
+ *                      as a sum of two, and 1 / sqrt(var + eps)).
+ * nerf_layer_norm_bwd: from the same x, w and stats: dx (or NULL), dw and db ([c] of w_type, either may be NULL), the latter
+ *                      summed over slices of the rows in fixed order (bitwise reproducible); workspace:
+ *                      nerf_layer_norm_workspace_floats(n, c) floats, contents irrelevant (may be NULL without dw and db). */
+#define NERF_LAYER_NORM_MAX_C (1 << 24)
+int nerf_layer_norm_fwd(int64_t n, int64_t c, int type, const void* x, int64_t ldx, int w_type, const void* w, const void* b,
+                        double eps, void* y, int64_t ldy, float* stats, void* stream);
+int64_t nerf_layer_norm_workspace_floats(int64_t n, int64_t c);
+int nerf_layer_norm_bwd(int64_t n, int64_t c, int type, const void* x, int64_t ldx, const void* dy, int64_t lddy, int w_type,
+                        const void* w, const float* stats, void* dx, int64_t lddx, void* dw, void* db, float* workspace,
+                        void* stream);
+
+/* Products in 8 bits with a power-of-two scale per row and 128 values of k (ops.linear_fp8; no counterpart upstream).
+ * A quantised matrix [rows, k]: codes, e4m3 bytes with a row stride of nerf_fp8_code_stride(k) bytes (k rounded up to a multiple
+ * of 128; the bytes behind k are zero), and scales, one byte e + 127 per row and block of 128 with a row stride of
+ * nerf_fp8_scale_stride(k) bytes (the number of blocks rounded up to a multiple of 4): a value is code * 2^e.  Codes start at a
+ * multiple of 16 bytes, scales of 4.
+ * nerf_fp8_quantize: x [rows, cols] of `type`, row stride ldx -> codes / scales of x (both or neither NULL) and codes_t /
+ *   scales_t of its transpose (both or neither NULL), every value rounded to nearest even once, e the smallest exponent (>= -126)
+ *   with max |x| <= 448 * 2^e over the block; a value that is not finite becomes NaN and has no part in its block's scale.  mask
+ *   (or NULL; of `type`, row stride ldm): x counts as 0 where mask <= 0.  col_sum (or NULL): [cols] of sum_type, the sums of the
+ *   columns of the (masked) x; it takes a workspace of nerf_fp8_quantize_workspace_floats(rows, cols) floats.
+ * nerf_fp8_matmul: c [m, n] of `type`, row stride ldc, = act(a [m, k] b [n, k]^T + bias [n]); bias (of bias_type: `type` or
+ *   NERF_F32) may be NULL; relu != 0 applies max(., 0) (a NaN stays).  Sums in fp32: for an fp32 c by the bf16 matrix instruction
+ *   on decoded values (products exact), for a 16-bit c by the scaled fp8 instruction, which cuts the products of eight consecutive
+ *   k to multiples of 2^-13 of the largest one's power of two (typically 1.5e-5 of the result).
+ *   workspace: nerf_fp8_matmul_workspace_floats(m, n, k, type) floats (0: may be NULL). */
+int64_t nerf_fp8_code_stride(int64_t k);
+int64_t nerf_fp8_scale_stride(int64_t k);
+int64_t nerf_fp8_quantize_workspace_floats(int64_t rows, int64_t cols);
+int nerf_fp8_quantize(int64_t rows, int64_t cols, int type, const void* x, int64_t ldx, const void* mask, int64_t ldm,
+                      uint8_t* codes, uint8_t* scales, uint8_t* codes_t, uint8_t* scales_t, int sum_type, void* col_sum,
+                      float* workspace, void* stream);
+int64_t nerf_fp8_matmul_workspace_floats(int64_t m, int64_t n, int64_t k, int type);
+int nerf_fp8_matmul(int64_t m, int64_t n, int64_t k, const uint8_t* a, const uint8_t* a_scales, const uint8_t* b,
+                    const uint8_t* b_scales, int bias_type, const void* bias, int relu, int type, void* c, int64_t ldc,
+                    float* workspace, void* stream);
+
+/* AdamW (decoupled weight decay) over n_tensors tensors anywhere in memory, all of `type`, in place (optim.AdamW; upstream
+ * has Adam only).  All pointers in the arrays are DEVICE, the arrays themselves and counts HOST.  Tensor i: counts[i] elements
+ * at params[i], gradients at grads[i], *steps[i] (a float) the number of updates taken so far, incremented by the call:
+ *   m += (1 - beta1)(g - m), v += (1 - beta2)(g g - v), p -= lr wd p + lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps).
+ * state_bits 32: exp_avg[i], exp_avg_sq[i] are fp32.  state_bits 8: exp_avg[i] e4m3 and exp_avg_sq[i] e5m2 bytes, scales[i] two
+ * floats (max |m| / 448, max v / 57344) per block of 128 consecutive elements; the states are rounded stochastically, from a hash
+ * of (element, step).  type 16-bit: masters[i] are fp32 copies the parameters are rounded from (an element of params that no
+ * longer equals its rounded master is taken as it is).  Tensors must not overlap.  lr_dev: the learning rate as a DEVICE float, or NULL and `lr` is used.
+ * workspace: nerf_adamw_workspace_floats(n_tensors) floats, 16-byte aligned.  One launch per NERF_ADAMW_BATCH tensors and
+ * one small one before it. */
+#define NERF_ADAMW_BATCH 60
+int64_t nerf_adamw_workspace_floats(int n_tensors);
+int nerf_adamw_step(int n_tensors, const int64_t* counts, int type, int state_bits, void* const* params,
+                    const void* const* grads, void* const* exp_avg, void* const* exp_avg_sq, float* const* scales,
+                    float* const* masters, float* const* steps, const float* lr_dev, double lr, double beta1, double beta2,
+                    double eps, double weight_decay, float* workspace, void* stream);
 
 /* nerf_mlp_bwd_bf16x3 for callers that cannot allocate device memory (code under HIP graph capture, tight serving
  * loops, harnesses that forbid hipMalloc): no counterpart upstream.  Same arguments and results, bit for bit, minus

@@ -92,6 +92,17 @@ SIGNATURES = {
     "nerf_linear_bwd_data": (_i, [_l, _i, _i, _p, _l, _p, _p, _l, _p]),
     "nerf_linear_workspace_floats": (_l, [_i, _i]),
     "nerf_linear_bwd_weights": (_i, [_l, _i, _i, _p, _l, _p, _l, _p, _p, _p, _p]),
+    "nerf_layer_norm_fwd": (_i, [_l, _l, _i, _p, _l, _i, _p, _p, _d, _p, _l, _p, _p]),
+    "nerf_layer_norm_workspace_floats": (_l, [_l, _l]),
+    "nerf_layer_norm_bwd": (_i, [_l, _l, _i, _p, _l, _p, _l, _i, _p, _p, _p, _l, _p, _p, _p, _p]),
+    "nerf_fp8_code_stride": (_l, [_l]),
+    "nerf_fp8_scale_stride": (_l, [_l]),
+    "nerf_fp8_quantize_workspace_floats": (_l, [_l, _l]),
+    "nerf_fp8_quantize": (_i, [_l, _l, _i, _p, _l, _p, _l, _p, _p, _p, _p, _i, _p, _p, _p]),
+    "nerf_fp8_matmul_workspace_floats": (_l, [_l, _l, _l, _i]),
+    "nerf_fp8_matmul": (_i, [_l, _l, _l, _p, _p, _p, _p, _i, _p, _i, _i, _p, _l, _p, _p]),
+    "nerf_adamw_workspace_floats": (_l, [_i]),
+    "nerf_adamw_step": (_i, [_i, _p, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _d, _d, _d, _d, _d, _p, _p]),
     "nerf_mlp_bwd_static_max_points": (_l, []),
     "nerf_mlp_bwd_bf16x3_static": (_i, [_l, _p, _p, _i, _i, _p, _p, _p, _p]),
     "nerf_mlp_packed_bf16_bytes": (_l, [_i]),

@@ -1,0 +1,42 @@
+// Element types of the layer and optimiser operators (fp32, bf16, fp16): what is read is widened to fp32, what is written is
+// rounded to nearest even once.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <cstdint>
+
+namespace nerfhip {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+template <typename T> struct ElemTraits;
+template <> struct ElemTraits<float> { static constexpr int code = 0; };
+template <> struct ElemTraits<bf16_t> { static constexpr int code = 1; };
+template <> struct ElemTraits<f16_t> { static constexpr int code = 2; };
+
+inline int elem_size(int type) { return type == 0 ? 4 : 2; }
+inline bool elem_type_ok(int type) { return type >= 0 && type <= 2; }
+
+// N consecutive elements: one load or store of up to 16 bytes each; the address is a multiple of the vector's size (or of 16)
+template <typename T, int N>
+struct __attribute__((aligned(sizeof(T) * N > 16 ? 16 : sizeof(T) * N))) Vec {
+    T e[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void load_vec(const T* p, float (&out)[N]) {
+    const Vec<T, N> v = *reinterpret_cast<const Vec<T, N>*>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = (float)v.e[i];
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_vec(T* p, const float (&in)[N]) {
+    Vec<T, N> v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v.e[i] = (T)in[i];
+    *reinterpret_cast<Vec<T, N>*>(p) = v;
+}
+
+}  // namespace nerfhip

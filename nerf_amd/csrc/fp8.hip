@@ -1,0 +1,344 @@
+// Products of matrices held in 8 bits (e4m3) with one power-of-two scale per row and 128 values of k:
+//   C[i][j] = sum over blocks kb of 2^(ea[i][kb] + eb[j][kb]) sum over k in kb of a[i][k] b[j][k]   (+ bias[j], ReLU)
+// and the quantisation that makes the operands.  A scale is the smallest power of two that takes its block's largest value to at
+// most 448: x 2^-e is exact, so every value is rounded once, and the matrix instruction's own scale operands (E8M0 bytes, e + 127)
+// apply it inside the instruction.
+//
+// Which instruction multiplies goes by the output's type.  v_mfma_scale_f32_16x16x128_f8f6f4 cuts the products of every eight
+// consecutive k to multiples of 2^(E - 13), E the exponent of the largest of them (measured with one large product among small
+// ones), before it sums them in fp32: 1.1e-5 .. 1.8e-5 of the sum on normally distributed values (k = 128 .. 65536; the
+// unscaled fp8 instruction the same), which a 16-bit output, rounded to 2^-9 or 2^-12, does not show.  An fp32 output does: there
+// the codes are decoded to bf16 with their scale (exact: 4 bits into 8, the exponent range is fp32's) and multiplied by the
+// bf16 instruction, whose sums are within 4e-7.
+#include "common.hpp"
+#include "elem.hpp"
+#include "wave_ops.hpp"
+
+using namespace nerfhip;
+
+namespace {
+
+constexpr int KB = 128;       // values of k that share a scale
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+inline int64_t blocks_of(int64_t k) { return (k + KB - 1) / KB; }
+inline int64_t code_stride(int64_t k) { return blocks_of(k) * KB; }
+inline int64_t scale_stride(int64_t k) { return (blocks_of(k) + 3) / 4 * 4; }
+
+// ---- quantisation ---------------------------------------------------------------------------------------------------------------
+template <int CTRL>
+__device__ __forceinline__ unsigned max_ror(unsigned v) {
+    const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
+    return o > v ? o : v;
+}
+__device__ __forceinline__ unsigned row16_max(unsigned v) {
+    v = max_ror<0x121>(v);      // row_ror:1, 2, 4, 8 inside 16 lanes
+    v = max_ror<0x122>(v);
+    v = max_ror<0x124>(v);
+    return max_ror<0x128>(v);
+}
+
+// bits of |v| for the largest of a block; what is not finite has no part in it
+__device__ __forceinline__ unsigned mag_bits(float v) {
+    const unsigned u = __float_as_uint(v) & 0x7fffffffu;
+    return u < 0x7f800000u ? u : 0u;
+}
+// smallest e >= -126 with amax <= 448 * 2^e, from amax's bits (448 = 1.75 * 2^8)
+__device__ __forceinline__ int scale_exp(unsigned amax) {
+    const int e = (int)(amax >> 23) - 127 - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return e < -126 ? -126 : e;
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }      // -126 <= e <= 127
+// x * inv in e4m3, four to a word; what is not finite becomes NaN
+__device__ __forceinline__ float finite_or_nan(float v) {
+    return (__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u ? v : __uint_as_float(0x7fc00000u);
+}
+__device__ __forceinline__ unsigned pack4(float a, float b, float c, float d, float inv) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(finite_or_nan(a) * inv, finite_or_nan(b) * inv, 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(finite_or_nan(c) * inv, finite_or_nan(d) * inv, w, true);
+}
+
+constexpr int QT = 128;       // a workgroup quantises a tile of 128 x 128
+constexpr int QLD = QT + 1;
+
+// codes / scales: along the columns (rows keep their order); codes_t / scales_t: of the transpose, along the rows; colsum: sums of the
+// tile's columns, [tile row][cols].  mask: values whose mask entry is <= 0 count as 0 (the gradient of a ReLU's output).
+template <typename T, bool ROWS, bool COLS>
+__global__ void __launch_bounds__(256) k_quantize(int64_t rows, int64_t cols, const T* __restrict__ x, int64_t ldx, int wide,
+                                                  const T* __restrict__ mask, int64_t ldm, uint8_t* __restrict__ codes, int64_t ldc,
+                                                  uint8_t* __restrict__ scales, int64_t lds, uint8_t* __restrict__ codes_t, int64_t ldct,
+                                                  uint8_t* __restrict__ scales_t, int64_t ldst, float* __restrict__ colsum) {
+    extern __shared__ float tile[];       // [QT][QLD], only with COLS
+    const int64_t r0 = (int64_t)blockIdx.x * QT;
+    const int64_t c0 = (int64_t)blockIdx.y * QT;
+    const int tid = threadIdx.x, cl = (tid & 15) * 8;
+    const int64_t c = c0 + cl;
+#pragma unroll 2
+    for (int q = 0; q < 8; ++q) {
+        const int rl = (tid >> 4) + 16 * q;
+        const int64_t r = r0 + rl;
+        float v[8];
+        if (r < rows && wide && c + 8 <= cols) {
+            load_vec<T, 8>(x + r * ldx + c, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (r < rows && c + e < cols) ? (float)x[r * ldx + c + e] : 0.0f;
+        }
+        if (mask) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (r < rows && c + e < cols && (float)mask[r * ldm + c + e] <= 0.0f) v[e] = 0.0f;
+        }
+        if (COLS) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) tile[rl * QLD + cl + e] = v[e];
+        }
+        if (ROWS) {
+            unsigned am = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { const unsigned u = mag_bits(v[e]); am = u > am ? u : am; }
+            const int ex = scale_exp(row16_max(am));
+            const float inv = pow2(-ex);
+            if (r < rows) {
+                const uint2 w = make_uint2(pack4(v[0], v[1], v[2], v[3], inv), pack4(v[4], v[5], v[6], v[7], inv));
+                *reinterpret_cast<uint2*>(codes + r * ldc + c) = w;
+                if ((tid & 15) == 0) {
+                    scales[r * lds + blockIdx.y] = (uint8_t)(ex + 127);
+                    if (blockIdx.y + 1 == gridDim.y)
+                        for (int64_t z = blockIdx.y + 1; z < lds; ++z) scales[r * lds + z] = 0;
+                }
+            }
+        }
+    }
+    if (!COLS) return;
+    __syncthreads();
+    const int col = tid >> 1, half = tid & 1;       // two neighbouring lanes share a column
+    const int64_t gc = c0 + col;
+    unsigned am = 0;
+    float sum = 0.0f;
+#pragma unroll 8
+    for (int k = 0; k < 64; ++k) {
+        const float v = tile[(64 * half + k) * QLD + col];
+        const unsigned u = mag_bits(v);
+        am = u > am ? u : am;
+        sum += v;
+    }
+    const unsigned am2 = (unsigned)__shfl_xor((int)am, 1);
+    sum += __shfl_xor(sum, 1);
+    am = am2 > am ? am2 : am;
+    if (gc >= cols) return;
+    if (colsum && half == 0) colsum[(int64_t)blockIdx.x * cols + gc] = sum;
+    if (!codes_t) return;
+    const int ex = scale_exp(am);
+    const float inv = pow2(-ex);
+    uint8_t* dst = codes_t + gc * ldct + r0 + 64 * half;
+#pragma unroll
+    for (int k = 0; k < 64; k += 16) {
+        unsigned w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float* t = tile + (64 * half + k + 4 * j) * QLD + col;
+            w[j] = pack4(t[0], t[QLD], t[2 * QLD], t[3 * QLD], inv);
+        }
+        *reinterpret_cast<uint4*>(dst + k) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (half == 0) {
+        scales_t[gc * ldst + blockIdx.x] = (uint8_t)(ex + 127);
+        if (blockIdx.x + 1 == gridDim.x)
+            for (int64_t z = blockIdx.x + 1; z < ldst; ++z) scales_t[gc * ldst + z] = 0;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_colsum_finish(int64_t tiles, int64_t cols, const float* __restrict__ part, T* __restrict__ out) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= cols) return;
+    double s = 0.0;
+    for (int64_t t = 0; t < tiles; ++t) s += (double)part[t * cols + c];
+    out[c] = (T)(float)s;
+}
+
+// ---- products -------------------------------------------------------------------------------------------------------------------
+struct Product {
+    const uint8_t *a, *b, *sa, *sb;
+    int64_t m, n;
+    int64_t ldk, lds;         // row strides of codes and scales
+    int blocks;               // 128-blocks of k
+    const void* bias;
+    int bias_f32, relu;
+    void* c;
+    int64_t ldc;
+};
+
+template <typename T>
+__device__ __forceinline__ float finish(float v, const Product& p, int64_t col) {
+    if (p.bias) v += p.bias_f32 ? ((const float*)p.bias)[col] : (float)((const T*)p.bias)[col];
+    if (p.relu) v = v > 0.0f ? v : (v != v ? v : 0.0f);      // keeps a NaN
+    return v;
+}
+
+__device__ __forceinline__ i32x8 load32(const uint8_t* p) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p), y = *reinterpret_cast<const uint4*>(p + 16);
+    i32x8 r;
+    r[0] = x.x; r[1] = x.y; r[2] = x.z; r[3] = x.w; r[4] = y.x; r[5] = y.y; r[6] = y.z; r[7] = y.w;
+    return r;
+}
+
+// acc += a b^T over one block of k: a lane holds 32 of the 128 values of row (lane & 15) of either operand, and that row's scale byte
+__device__ __forceinline__ f32x4 mul_fp8(i32x8 a, int sa, i32x8 b, int sb, f32x4 acc) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 0, 0, 0, sa, 0, sb);
+}
+__device__ __forceinline__ bf16x8 decode8(int lo, int hi, float scale) {
+    const bf16x2 p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), q = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+    const bf16x2 r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), s = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+    return bf16x8{p[0], p[1], q[0], q[1], r[0], r[1], s[0], s[1]};
+}
+__device__ __forceinline__ f32x4 mul_decoded(i32x8 a, int sa, i32x8 b, int sb, f32x4 acc) {
+    const float fa = __uint_as_float((unsigned)sa << 23), fb = __uint_as_float((unsigned)sb << 23);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(decode8(a[2 * q], a[2 * q + 1], fa), decode8(b[2 * q], b[2 * q + 1], fb), acc, 0, 0, 0);
+    return acc;
+}
+
+// Few rows: a workgroup owns 16 columns of C and up to 16 MT rows; its waves take the blocks of k in turn, straight from memory into the
+// instruction's registers, and add up through LDS.
+constexpr int FEW_WAVES = 8;
+template <typename T, int MT>
+__global__ void __launch_bounds__(64 * FEW_WAVES) k_product_few(Product p) {
+    constexpr bool F32 = sizeof(T) == 4;
+    __shared__ f32x4 red[FEW_WAVES][MT][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    const int64_t j0 = (int64_t)blockIdx.x * 16, i0 = (int64_t)blockIdx.y * 16 * MT;
+    const int64_t jb = j0 + r < p.n ? j0 + r : p.n - 1;
+    const uint8_t *bp = p.b + jb * p.ldk + 32 * g, *sbp = p.sb + jb * p.lds;
+    const uint8_t *ap[MT], *sap[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int64_t ia = i0 + 16 * t + r < p.m ? i0 + 16 * t + r : p.m - 1;
+        ap[t] = p.a + ia * p.ldk + 32 * g;
+        sap[t] = p.sa + ia * p.lds;
+    }
+    f32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0, 0, 0, 0};
+    for (int kb = wave; kb < p.blocks; kb += FEW_WAVES) {
+        const i32x8 b = load32(bp + (int64_t)kb * KB);
+        const int sb = sbp[kb];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const i32x8 a = load32(ap[t] + (int64_t)kb * KB);
+            const int sa = sap[t][kb];
+            acc[t] = F32 ? mul_decoded(a, sa, b, sb, acc[t]) : mul_fp8(a, sa, b, sb, acc[t]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) red[wave][t][lane] = acc[t];
+    __syncthreads();
+    for (int t = wave; t < MT; t += FEW_WAVES) {
+        f32x4 s = red[0][t][lane];
+#pragma unroll
+        for (int w = 1; w < FEW_WAVES; ++w) s += red[w][t][lane];
+        const int64_t col = j0 + r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t row = i0 + 16 * t + 4 * g + e;
+            if (row < p.m && col < p.n) ((T*)p.c)[row * p.ldc + col] = (T)finish<T>(s[e], p, col);
+        }
+    }
+}
+
+template <typename T>
+int product(const Product& p, hipStream_t stream) {
+    constexpr int MT = 4;
+    const int64_t gx = (p.n + 15) / 16, gy = (p.m + 16 * MT - 1) / (16 * MT);
+    if (gx > 0x7fffff || gy > 65535) return fail(NERF_E_ARG, "nerf_fp8_matmul: %lld x %lld is more than one launch covers", (long long)p.m, (long long)p.n);
+    hipLaunchKernelGGL((k_product_few<T, MT>), dim3((unsigned)gx, (unsigned)gy), dim3(64 * FEW_WAVES), 0, stream, p);
+    return launched("nerf_fp8_matmul");
+}
+
+template <typename T>
+int quantize(int64_t rows, int64_t cols, const T* x, int64_t ldx, const T* mask, int64_t ldm, uint8_t* codes, uint8_t* scales,
+             uint8_t* codes_t, uint8_t* scales_t, int sum_type, void* col_sum, float* ws, hipStream_t stream) {
+    const int64_t ldc = code_stride(cols), lds = scale_stride(cols), ldct = code_stride(rows), ldst = scale_stride(rows);
+    const dim3 grid((unsigned)((rows + QT - 1) / QT), (unsigned)((cols + QT - 1) / QT));
+    const int wide = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(ldx * sizeof(T))) & 15) == 0;
+    const size_t bytes = sizeof(float) * QT * QLD;
+    const bool cols_too = codes_t || col_sum;
+#define GO(R, C)                                                                                                                     \
+    do {                                                                                                                             \
+        if (C) {                                                                                                                     \
+            const hipError_t e = lds_limit_once((const void*)&k_quantize<T, R, C>, bytes);                                           \
+            if (e != hipSuccess) return fail(NERF_E_LAUNCH, "nerf_fp8_quantize: %s", hipGetErrorString(e));                          \
+        }                                                                                                                            \
+        hipLaunchKernelGGL((k_quantize<T, R, C>), grid, dim3(256), C ? bytes : 0, stream, rows, cols, x, ldx, wide, mask, ldm, codes, ldc, \
+                           scales, lds, codes_t, ldct, scales_t, ldst, col_sum ? ws : (float*)nullptr);                              \
+    } while (0)
+    if (codes && cols_too) GO(true, true); else if (codes) GO(true, false); else GO(false, true);
+#undef GO
+    const int rc = launched("nerf_fp8_quantize");
+    if (rc || !col_sum) return rc;
+    const dim3 cgrid((unsigned)((cols + 255) / 256));
+    const int64_t tiles = (rows + QT - 1) / QT;
+    if (sum_type == NERF_F32) hipLaunchKernelGGL((k_colsum_finish<float>), cgrid, dim3(256), 0, stream, tiles, cols, ws, (float*)col_sum);
+    else hipLaunchKernelGGL((k_colsum_finish<T>), cgrid, dim3(256), 0, stream, tiles, cols, ws, (T*)col_sum);
+    return launched("nerf_fp8_quantize (sums)");
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t nerf_fp8_code_stride(int64_t k) { return k < 1 ? 0 : code_stride(k); }
+int64_t nerf_fp8_scale_stride(int64_t k) { return k < 1 ? 0 : scale_stride(k); }
+int64_t nerf_fp8_quantize_workspace_floats(int64_t rows, int64_t cols) { return rows < 1 || cols < 1 ? 0 : (rows + QT - 1) / QT * cols; }
+
+int nerf_fp8_quantize(int64_t rows, int64_t cols, int type, const void* x, int64_t ldx, const void* mask, int64_t ldm, uint8_t* codes,
+                      uint8_t* scales, uint8_t* codes_t, uint8_t* scales_t, int sum_type, void* col_sum, float* workspace, void* stream_) {
+    NERF_REQUIRE(!col_sum || sum_type == type || sum_type == NERF_F32, "nerf_fp8_quantize: type=%d sum_type=%d", type, sum_type);
+    NERF_REQUIRE(rows >= 0 && cols >= 1, "nerf_fp8_quantize: rows=%lld cols=%lld", (long long)rows, (long long)cols);
+    NERF_REQUIRE(elem_type_ok(type), "nerf_fp8_quantize: type=%d", type);
+    NERF_REQUIRE(rows <= (int64_t)QT * 0x7fffff && cols <= (int64_t)QT * 65535, "nerf_fp8_quantize: %lld x %lld is more than one launch covers",
+                 (long long)rows, (long long)cols);
+    NERF_REQUIRE(rows <= 1 || (ldx >= cols && (!mask || ldm >= cols)), "nerf_fp8_quantize: a row stride is less than cols=%lld", (long long)cols);
+    if (rows == 0) return 0;
+    NERF_REQUIRE(x && (!codes == !scales) && (!codes_t == !scales_t) && (codes || codes_t || col_sum) && (!col_sum || workspace),
+                 "nerf_fp8_quantize: null pointer");
+    NERF_REQUIRE(((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(codes_t)) & 15) == 0,
+                 "nerf_fp8_quantize: codes start at a multiple of 16 bytes");
+    hipStream_t stream = as_stream(stream_);
+#define GO(T) return quantize<T>(rows, cols, (const T*)x, ldx, (const T*)mask, ldm, codes, scales, codes_t, scales_t, sum_type, col_sum, workspace, stream)
+    if (type == NERF_F32) GO(float);
+    if (type == NERF_BF16) GO(bf16_t);
+    GO(f16_t);
+#undef GO
+}
+
+int nerf_fp8_matmul(int64_t m, int64_t n, int64_t k, const uint8_t* a, const uint8_t* a_scales, const uint8_t* b, const uint8_t* b_scales,
+                    int bias_type, const void* bias, int relu, int type, void* c, int64_t ldc, float* workspace, void* stream_) {
+    NERF_REQUIRE(m >= 0 && n >= 0 && k >= 1 && k <= 0x7fffffff, "nerf_fp8_matmul: m=%lld n=%lld k=%lld", (long long)m, (long long)n, (long long)k);
+    NERF_REQUIRE(elem_type_ok(type) && (!bias || bias_type == type || bias_type == NERF_F32), "nerf_fp8_matmul: type=%d bias_type=%d", type, bias_type);
+    NERF_REQUIRE(m <= 1 || ldc >= n, "nerf_fp8_matmul: ldc=%lld is less than n=%lld", (long long)ldc, (long long)n);
+    if (m == 0 || n == 0) return 0;
+    NERF_REQUIRE(a && a_scales && b && b_scales && c, "nerf_fp8_matmul: null pointer");
+    NERF_REQUIRE(((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0 &&
+                 ((reinterpret_cast<uintptr_t>(a_scales) | reinterpret_cast<uintptr_t>(b_scales)) & 3) == 0,
+                 "nerf_fp8_matmul: codes start at a multiple of 16 bytes, scales of 4");
+    (void)workspace;
+    Product p{a, b, a_scales, b_scales, m, n, code_stride(k), scale_stride(k), (int)blocks_of(k), bias, bias_type == NERF_F32, relu, c, ldc};
+    hipStream_t stream = as_stream(stream_);
+    if (type == NERF_F32) return product<float>(p, stream);
+    if (type == NERF_BF16) return product<bf16_t>(p, stream);
+    return product<f16_t>(p, stream);
+}
+
+int64_t nerf_fp8_matmul_workspace_floats(int64_t m, int64_t n, int64_t k, int type) {
+    (void)m; (void)n; (void)k; (void)type;
+    return 0;
+}
+
+}  // extern "C"

@@ -904,3 +904,234 @@ class _Linear(torch.autograd.Function):
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], relu: bool = False) -> torch.Tensor:
     """torch.nn.functional.linear (+ optional ReLU) on the library's own matrix kernel, differentiable in x, weight, bias."""
     return _Linear.apply(x, weight, bias, relu)
+
+
+# ------------------------------------------------------------------------------------------------
+# layers of wide networks: layer norm, products in 8 bits
+# ------------------------------------------------------------------------------------------------
+ELEM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # NERF_F32, NERF_BF16, NERF_F16
+
+
+def _elem(t: torch.Tensor, what: str) -> int:
+    code = ELEM_TYPES.get(t.dtype)
+    if code is None or not t.is_cuda:
+        raise TypeError(f"{what}: expected an fp32, bf16 or fp16 tensor on a HIP device, got {t.dtype} on {t.device}")
+    return code
+
+
+def _rows_any(t: torch.Tensor, what: str) -> torch.Tensor:
+    """[..., c] of any of the three types -> a 2-d view whose rows are contiguous (row stride >= c), or a copy."""
+    _elem(t, what)
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError(f"{what}: expected at least one value in the last dimension, got shape {tuple(t.shape)}")
+    t2 = t.reshape(-1, t.shape[-1])
+    if t2.stride(1) != 1 or (t2.shape[0] > 1 and t2.stride(0) < t2.shape[1]):
+        t2 = t2.contiguous()
+    return t2
+
+
+def _vector(t: Optional[torch.Tensor], size: int, like: torch.Tensor, what: str) -> Optional[torch.Tensor]:
+    """A bias or a norm's weight: [size], in `like`'s type or fp32, on its device."""
+    if t is None:
+        return None
+    if tuple(t.shape) != (size,):
+        raise ValueError(f"{what}: expected shape ({size},), got {tuple(t.shape)}")
+    if t.device != like.device or t.dtype not in (like.dtype, torch.float32):
+        raise TypeError(f"{what}: expected {like.dtype} or fp32 on {like.device}, got {t.dtype} on {t.device}")
+    return t.contiguous()
+
+
+class _LayerNorm(torch.autograd.Function):
+    """Layer norm over the last dimension, forward and backward in libnerf_hip.so (layer_norm.hip)."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, eps, need_grad):
+        x2 = _rows_any(x, "x")
+        n, c = x2.shape
+        wc, bc = _vector(w, c, x2, "weight"), _vector(b, c, x2, "bias")
+        if wc is not None and bc is not None and wc.dtype != bc.dtype:
+            raise TypeError(f"layer_norm: weight is {wc.dtype}, bias {bc.dtype}")
+        w_type = _elem(wc if wc is not None else bc if bc is not None else x2, "weight")
+        y = torch.empty((n, c), dtype=x.dtype, device=x2.device)
+        stats = torch.empty((3, n), dtype=torch.float32, device=x2.device) if need_grad else None
+        with torch.cuda.device(x2.device), _timed("layer_norm", 2 * n * c * x2.element_size()):
+            check(lib.nerf_layer_norm_fwd(n, c, ELEM_TYPES[x2.dtype], x2.data_ptr(), _ld(x2), w_type, _ptr(wc), _ptr(bc), eps,
+                                          y.data_ptr(), c, _ptr(stats), _stream()))
+        ctx.save_for_backward(x2, wc, stats)
+        ctx.lead, ctx.w_type = tuple(x.shape[:-1]), w_type
+        return y.reshape(ctx.lead + (c,))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x2, wc, stats = ctx.saved_tensors
+        n, c = x2.shape
+        dy2 = _rows_any(dy, "grad")
+        dev = x2.device
+        w_dtype = {v: k for k, v in ELEM_TYPES.items()}[ctx.w_type]
+        dx = torch.empty((n, c), dtype=x2.dtype, device=dev) if ctx.needs_input_grad[0] else None
+        dw = torch.empty((c,), dtype=w_dtype, device=dev) if ctx.needs_input_grad[1] else None
+        db = torch.empty((c,), dtype=w_dtype, device=dev) if ctx.needs_input_grad[2] else None
+        ws = None
+        if dw is not None or db is not None:
+            ws = torch.empty(lib.nerf_layer_norm_workspace_floats(n, c), dtype=torch.float32, device=dev)
+        with torch.cuda.device(dev), _timed("layer_norm_bwd", 3 * n * c * x2.element_size()):
+            check(lib.nerf_layer_norm_bwd(n, c, ELEM_TYPES[x2.dtype], x2.data_ptr(), _ld(x2), dy2.data_ptr(), _ld(dy2), ctx.w_type,
+                                          _ptr(wc), _ptr(stats), _ptr(dx), c, _ptr(dw), _ptr(db), _ptr(ws), _stream()))
+        return None if dx is None else dx.reshape(ctx.lead + (c,)), dw, db, None, None
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """torch.nn.functional.layer_norm over the last dimension, differentiable once in x, weight and bias.  x: fp32, bf16 or fp16,
+    rows of any stride; weight, bias: [x.shape[-1]], x's type or fp32, both alike.  Statistics in fp32; the weight's and bias's
+    gradients are summed in a fixed order (bitwise reproducible)."""
+    if not eps >= 0.0:
+        raise ValueError(f"layer_norm: eps={eps}")
+    need = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias))
+    return _LayerNorm.apply(x, weight, bias, float(eps), need)
+
+
+class Fp8Rows:
+    """A matrix [rows, k] held in 8 bits along k: `codes`, float8_e4m3fn [rows, k rounded up to a multiple of 128] with zeros
+    behind k, and `scales`, uint8 [rows, number of 128-blocks rounded up to a multiple of 4], the exponent of each block's
+    power-of-two scale plus 127: value = code * 2^(scale - 127).  quantize_fp8 makes one; weights kept in 8 bits are wrapped
+    directly."""
+    __slots__ = ("codes", "scales", "rows", "k")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, k: int):
+        k = int(k)
+        if k < 1 or codes.dim() != 2 or scales.dim() != 2:
+            raise ValueError(f"Fp8Rows: k={k}, codes {tuple(codes.shape)}, scales {tuple(scales.shape)}")
+        if codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.uint8:
+            raise TypeError(f"Fp8Rows: expected float8_e4m3fn codes and uint8 scales, got {codes.dtype} and {scales.dtype}")
+        rows = codes.shape[0]
+        want = (rows, int(lib.nerf_fp8_code_stride(k))), (rows, int(lib.nerf_fp8_scale_stride(k)))
+        if (tuple(codes.shape), tuple(scales.shape)) != want:
+            raise ValueError(f"Fp8Rows: for k={k} expected codes {want[0]} and scales {want[1]}, got {tuple(codes.shape)} and "
+                             f"{tuple(scales.shape)}")
+        if not codes.is_cuda or codes.device != scales.device:
+            raise TypeError(f"Fp8Rows: expected tensors on one HIP device, got {codes.device} and {scales.device}")
+        if not (codes.is_contiguous() and scales.is_contiguous()) or codes.data_ptr() % 16 or scales.data_ptr() % 4:
+            raise ValueError("Fp8Rows: codes and scales must be contiguous and start at a multiple of 16 and 4 bytes")
+        self.codes, self.scales, self.rows, self.k = codes, scales, rows, k
+
+
+def _fp8_empty(rows: int, k: int, dev):
+    return (torch.empty((rows, int(lib.nerf_fp8_code_stride(k))), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn),
+            torch.empty((rows, int(lib.nerf_fp8_scale_stride(k))), dtype=torch.uint8, device=dev))
+
+
+def _quantize(x2: torch.Tensor, want: bool, want_t: bool, mask: Optional[torch.Tensor] = None, sum_dtype=None):
+    """x2 [rows, cols] -> (Fp8Rows of x2, Fp8Rows of its transpose, column sums), each None unless asked for; one pass over x2."""
+    rows, cols = x2.shape
+    dev = x2.device
+    q, qt, sums, ws = (None, None), (None, None), None, None
+    if want:
+        q = _fp8_empty(rows, cols, dev)
+    if want_t:
+        qt = _fp8_empty(cols, rows, dev)
+    if sum_dtype is not None:
+        sums = torch.empty((cols,), dtype=sum_dtype, device=dev)
+        ws = torch.empty(lib.nerf_fp8_quantize_workspace_floats(rows, cols), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev), _timed("fp8_quantize", rows * cols * (x2.element_size() + int(want) + int(want_t))):
+        check(lib.nerf_fp8_quantize(rows, cols, ELEM_TYPES[x2.dtype], x2.data_ptr(), _ld(x2), _ptr(mask), 0 if mask is None else _ld(mask),
+                                    _ptr(q[0]), _ptr(q[1]), _ptr(qt[0]), _ptr(qt[1]), 0 if sums is None else ELEM_TYPES[sum_dtype],
+                                    _ptr(sums), _ptr(ws), _stream()))
+    return Fp8Rows(*q, cols) if want else None, Fp8Rows(*qt, rows) if want_t else None, sums
+
+
+def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
+    """x [rows, k] (fp32, bf16 or fp16) in e4m3 with one power-of-two scale per row and 128 values of k: the smallest that takes
+    the block's largest value to at most 448, so that every value is rounded (to nearest even) once.  A value that is not finite
+    becomes NaN."""
+    if x.dim() != 2:
+        raise ValueError(f"quantize_fp8: expected a matrix, got shape {tuple(x.shape)}")
+    return _quantize(_rows_any(x.detach(), "x"), True, False)[0]
+
+
+def matmul_fp8(a: Fp8Rows, b: Fp8Rows, bias: Optional[torch.Tensor] = None, relu: bool = False,
+               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """a [m, k] b [n, k]^T + bias [n] (+ ReLU) in out_dtype (fp32, bf16 or fp16); sums in fp32."""
+    if not (isinstance(a, Fp8Rows) and isinstance(b, Fp8Rows)):
+        raise TypeError("matmul_fp8: expected two Fp8Rows")
+    if a.k != b.k:
+        raise ValueError(f"matmul_fp8: k={a.k} against k={b.k}")
+    if out_dtype not in ELEM_TYPES:
+        raise TypeError(f"matmul_fp8: out_dtype {out_dtype}")
+    dev = a.codes.device
+    if b.codes.device != dev:
+        raise TypeError(f"matmul_fp8: operands on {dev} and {b.codes.device}")
+    c = torch.empty((a.rows, b.rows), dtype=out_dtype, device=dev)
+    bias = _vector(bias, b.rows, c, "bias")
+    kind = ELEM_TYPES[out_dtype]
+    floats = lib.nerf_fp8_matmul_workspace_floats(a.rows, b.rows, a.k, kind)
+    ws = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
+    with torch.cuda.device(dev), _timed("fp8_matmul", 2 * a.rows * b.rows * a.k):
+        check(lib.nerf_fp8_matmul(a.rows, b.rows, a.k, a.codes.data_ptr(), a.scales.data_ptr(), b.codes.data_ptr(), b.scales.data_ptr(),
+                                  kind if bias is None else ELEM_TYPES[bias.dtype], _ptr(bias), int(bool(relu)), kind, c.data_ptr(),
+                                  b.rows, _ptr(ws), _stream()))
+    return c
+
+
+class _LinearFp8(torch.autograd.Function):
+    """y = act(q(x) q(w)^T + b); dx = q(dy) q(w^T)^T and dw = q(dy^T) q(x^T)^T, every operand quantised along its own k from the
+    unquantised values; what the backward pass needs of x and w is kept in 8 bits."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, relu, need_grad):
+        x2, w2 = _rows_any(x, "x"), _rows_any(w, "weight")
+        need_dx, need_dw = need_grad and ctx.needs_input_grad[0], need_grad and ctx.needs_input_grad[1]
+        xq, xt, _ = _quantize(x2, True, need_dw and x2.shape[0] > 0)
+        wq, wt, _ = _quantize(w2, True, need_dx)
+        y = matmul_fp8(xq, wq, b, relu, x2.dtype)
+        kept = [t for q in (xt, wt) if q is not None for t in (q.codes, q.scales)]
+        ctx.save_for_backward(*kept, *([y] if relu and need_grad else []))
+        ctx.kept = xt is not None, wt is not None, bool(relu)
+        ctx.lead, ctx.shape, ctx.w_dtype, ctx.b_dtype = tuple(x.shape[:-1]), (x2.shape[0],) + tuple(w2.shape), w.dtype, None if b is None else b.dtype
+        return y.reshape(ctx.lead + (w2.shape[0],))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        saved = list(ctx.saved_tensors)
+        n, n_out, n_in = ctx.shape
+        xt = Fp8Rows(saved.pop(0), saved.pop(0), n) if ctx.kept[0] else None
+        wt = Fp8Rows(saved.pop(0), saved.pop(0), n_out) if ctx.kept[1] else None
+        y = saved.pop(0) if ctx.kept[2] else None
+        dy2 = _rows_any(dy, "grad")
+        need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
+        dx = dw = db = None
+        if n == 0:
+            dx = torch.empty((0, n_in), dtype=dy.dtype, device=dy.device) if need_dx else None
+            dw = torch.zeros((n_out, n_in), dtype=ctx.w_dtype, device=dy.device) if need_dw else None
+            db = torch.zeros((n_out,), dtype=ctx.b_dtype, device=dy.device) if need_db else None
+        elif need_dx or need_dw or need_db:
+            gq, gt, db = _quantize(dy2, need_dx, need_dw, y, ctx.b_dtype if need_db else None)
+            if need_dx:
+                dx = matmul_fp8(gq, wt, out_dtype=dy2.dtype)
+            if need_dw:
+                dw = matmul_fp8(gt, xt, out_dtype=ctx.w_dtype)
+        return None if dx is None else dx.reshape(ctx.lead + (n_in,)), dw, db, None, None
+
+
+def linear_fp8(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = None, relu: bool = False) -> torch.Tensor:
+    """ops.linear with both operands of every product held in 8 bits, one power-of-two scale per row and 128 values of k.
+    x [..., k]: fp32, bf16 or fp16, and the result's type.  weight: a tensor [n, k] of x's type or fp32 -- quantised in the call,
+    differentiable once in x, weight and bias (each product of the backward pass in 8 bits as well) -- or an Fp8Rows (kept by a
+    program that only evaluates; no gradients).  Sums are fp32."""
+    if isinstance(weight, Fp8Rows):
+        if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+            raise ValueError("linear_fp8: a weight held in 8 bits has no backward pass; call it under torch.no_grad()")
+        x2 = _rows_any(x, "x")
+        if x2.shape[1] != weight.k:
+            raise ValueError(f"linear_fp8: x has {x2.shape[1]} values per row, the weight k={weight.k}")
+        y = matmul_fp8(_quantize(x2, True, False)[0], weight, bias, relu, x2.dtype)
+        return y.reshape(tuple(x.shape[:-1]) + (weight.rows,))
+    _elem(x, "x")
+    if weight.dim() != 2 or x.dim() < 1 or weight.shape[1] != x.shape[-1]:
+        raise ValueError(f"linear_fp8: x {tuple(x.shape)} against weight {tuple(weight.shape)}")
+    if weight.device != x.device or weight.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"linear_fp8: expected a weight in {x.dtype} or fp32 on {x.device}, got {weight.dtype} on {weight.device}")
+    need = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias))
+    return _LinearFp8.apply(x, weight, bias, relu, need)

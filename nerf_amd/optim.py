@@ -14,6 +14,8 @@ is not contiguous -- takes torch.optim.Adam.step() unchanged, on the same state.
 The step only enqueues work (learning rate and step count are read on the device when they live there), so it can be
 recorded into a HIP graph like the stock capturable optimiser -- after one eager step: the first step on a layout moves the
 moments into their buffers and reads one word back from the device.
+
+`AdamW` decouples the weight decay, takes tensors wherever they lie, and holds its states in 32 or in 8 bits.
 """
 from __future__ import annotations
 
@@ -23,6 +25,7 @@ from typing import List, Optional
 import torch
 
 from ._lib import check, lib
+from .ops import ELEM_TYPES
 
 
 class _Run:
@@ -199,3 +202,184 @@ class FlatAdam(torch.optim.Adam):
                 if st and "step" in st and not (torch.is_tensor(st["step"]) and st["step"].is_cuda):
                     st["step"] = torch.as_tensor(float(st["step"]), dtype=torch.float32, device=p.device)
         self._layout_key = None
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) over any tensors, wherever they lie: one launch of the library's kernel per 60 tensors of a
+    group, device and type, after a small one that counts the steps -- where FlatAdam needs parameters and gradients back to back.
+
+    Parameters are fp32, bf16 or fp16 and contiguous, on a HIP device when the step is taken.  `state[p]` holds ordinary tensors:
+      step         fp32 scalar on the device
+      exp_avg, exp_avg_sq   state_bits = 32: fp32, as torch.optim.AdamW's (whose checkpoints of fp32 parameters load, and the reverse);
+                   state_bits = 8: float8_e4m3fn and float8_e5m2, relative to `scale`
+      scale        state_bits = 8: fp32 [blocks of 128 consecutive elements, 2]: the largest |exp_avg| / 448 and exp_avg_sq / 57344
+      master       16-bit parameters: the fp32 values they are rounded from (an element of the parameter that was written from
+                   outside, and so is no longer its master's rounding, is taken as it is)
+    8-bit states are rounded stochastically from a hash of (element, step), so a run repeats bit for bit; a gradient that is not
+    finite reaches the states of its whole block of 128 (with 32 bits: of its element).  The learning rate may be a float or an fp32
+    device scalar, which a captured step reads at every replay; take one eager step before capturing."""
+
+    _MOMENTS = {32: (torch.float32, torch.float32), 8: (torch.float8_e4m3fn, torch.float8_e5m2)}
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32):
+        if state_bits not in self._MOMENTS:
+            raise ValueError(f"AdamW: state_bits={state_bits} is neither 32 nor 8")
+        self._check_hyper(lr, betas, eps, weight_decay)
+        self.state_bits = state_bits
+        self._slots = {}      # parameter -> (its state dict, the dict's tensors, their addresses): see _slot
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, capturable=True))
+
+    @staticmethod
+    def _check_hyper(lr, betas, eps, weight_decay):
+        if not torch.is_tensor(lr) and not lr >= 0.0:
+            raise ValueError(f"AdamW: lr={lr}")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f"AdamW: betas={betas}")
+        if not eps >= 0.0 or not weight_decay >= 0.0:
+            raise ValueError(f"AdamW: eps={eps}, weight_decay={weight_decay}")
+
+    def add_param_group(self, param_group):
+        params = param_group["params"]
+        params = [params] if torch.is_tensor(params) else list(params)
+        if len({id(p) for p in params}) != len(params):
+            raise ValueError("AdamW: a parameter appears twice in one group")
+        super().add_param_group({**param_group, "params": params})
+
+    # ---- states --------------------------------------------------------------------------------------
+    def _layout(self, p):
+        """name -> (type, shape) of the state of `p`."""
+        m, v = self._MOMENTS[self.state_bits]
+        out = {"step": (torch.float32, torch.Size(())), "exp_avg": (m, p.shape), "exp_avg_sq": (v, p.shape)}
+        if self.state_bits == 8:
+            out["scale"] = (torch.float32, torch.Size(((p.numel() + 127) // 128, 2)))
+        if p.dtype != torch.float32:
+            out["master"] = (torch.float32, p.shape)
+        return out
+
+    def _new_state(self, p):
+        out = {}
+        for name, (dtype, shape) in self._layout(p).items():
+            if name == "master":
+                out[name] = p.detach().to(torch.float32)
+            elif dtype.itemsize == 1:
+                out[name] = torch.zeros(shape, dtype=torch.uint8, device=p.device).view(dtype)
+            else:
+                out[name] = torch.zeros(shape, dtype=dtype, device=p.device)
+        return out
+
+    def _slot(self, p):
+        """The state's addresses, checked when a state is first seen: (dict, its tensors, exp_avg, exp_avg_sq, scale, master, step)."""
+        st = self.state[p]
+        if not st:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: take one eager step before capturing (the states would be made anew by every replay)")
+            st.update(self._new_state(p))
+        for name, (dtype, shape) in self._layout(p).items():
+            t = st.get(name)
+            if (not torch.is_tensor(t) or t.dtype != dtype or t.shape != shape or t.device != p.device or not t.is_contiguous()):
+                raise ValueError(f"AdamW: the state's {name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {p.device}, got "
+                                 f"{(t.dtype, tuple(t.shape), t.device) if torch.is_tensor(t) else t}")
+        names = ("exp_avg", "exp_avg_sq", "scale", "master", "step")
+        tensors = tuple(st.get(name) for name in names)
+        slot = (st, tensors, tuple(0 if t is None else t.data_ptr() for t in tensors), p.shape, p.dtype, p.device)
+        self._slots[p] = slot
+        return slot
+
+    def _current(self, p):
+        """The slot of `p`, made anew when its state or the parameter itself is no longer the one seen before."""
+        slot = self._slots.get(p)
+        if slot is not None:
+            st, (m, v, scale, master, step), _, shape, dtype, device = slot
+            if (self.state.get(p) is st and st.get("exp_avg") is m and st.get("exp_avg_sq") is v and st.get("step") is step
+                    and st.get("scale") is scale and st.get("master") is master
+                    and p.dtype is dtype and p.shape == shape and p.device == device):
+                return slot
+        return self._slot(p)
+
+    # ---- the step ------------------------------------------------------------------------------------
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work = []
+        for group in self.param_groups:
+            lists = {}      # (device, type) -> rows of (count, p, g, exp_avg, exp_avg_sq, scale, master, step)
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                if g.is_sparse or g.layout != torch.strided:
+                    raise TypeError("AdamW: sparse gradients are not supported")
+                if p.dtype not in ELEM_TYPES or not p.is_cuda:
+                    raise TypeError(f"AdamW: expected fp32, bf16 or fp16 parameters on a HIP device, got {p.dtype} on {p.device}")
+                if not p.is_contiguous():
+                    raise ValueError(f"AdamW: a parameter of shape {tuple(p.shape)} is not contiguous")
+                if g.dtype != p.dtype or g.device != p.device:
+                    raise TypeError(f"AdamW: a gradient in {g.dtype} on {g.device} for a parameter in {p.dtype} on {p.device}")
+                if not g.is_contiguous():
+                    g = g.contiguous()
+                lists.setdefault((p.device, p.dtype), []).append((p, g, self._current(p)))
+            work.append((group, lists))
+        for group, lists in work:
+            self._check_hyper(group["lr"], group["betas"], group["eps"], group["weight_decay"])
+            for (device, dtype), rows in lists.items():
+                self._launch(group, device, dtype, rows)
+        return loss
+
+    def _launch(self, group, device, dtype, rows):
+        n = len(rows)
+        lr, lr_dev = group["lr"], None
+        if torch.is_tensor(lr) and lr.is_cuda:
+            if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != device:
+                raise TypeError(f"AdamW: a device learning rate must be one fp32 value on {device}, got {lr.dtype} on {lr.device}")
+            lr_dev, lr = lr.data_ptr(), 0.0
+        pointers = ctypes.c_void_p * n
+        counts = (ctypes.c_int64 * n)(*[p.numel() for p, _, _ in rows])
+        params = pointers(*[p.data_ptr() for p, _, _ in rows])
+        grads = pointers(*[g.data_ptr() for _, g, _ in rows])
+        m, v, scale, master, step = [pointers(*column) for column in zip(*[slot[2] for _, _, slot in rows])]
+        with torch.cuda.device(device):
+            coef = torch.empty(lib.nerf_adamw_workspace_floats(n), dtype=torch.float32, device=device)
+            check(lib.nerf_adamw_step(n, counts, ELEM_TYPES[dtype], self.state_bits, params, grads, m, v, scale, master, step, lr_dev,
+                                      float(lr), float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]),
+                                      float(group["weight_decay"]), coef.data_ptr(), torch.cuda.current_stream().cuda_stream))
+
+    # ---- checkpoints ---------------------------------------------------------------------------------
+    def load_state_dict(self, state_dict):
+        """Checkpoints of this class with the same state_bits, and of torch.optim.Adam / AdamW with state_bits = 32.  The states keep
+        their own types (torch.optim would cast them to the parameter's)."""
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        fresh = {}
+        for i, p in zip(ids, params):
+            st = state_dict["state"].get(i)
+            if st is None:
+                continue
+            new = {}
+            for name, (dtype, shape) in self._layout(p).items():
+                t = st.get(name)
+                if name == "master" and t is None:
+                    new[name] = p.detach().to(torch.float32)
+                elif name == "step":
+                    new[name] = torch.as_tensor(0.0 if t is None else t, dtype=torch.float32).reshape(()).to(p.device).clone()
+                elif not torch.is_tensor(t) or t.dtype != dtype or t.shape != shape:
+                    raise ValueError(f"AdamW: with state_bits={self.state_bits} the checkpoint's {name} must be {dtype} of shape {tuple(shape)}, "
+                                     f"got {(t.dtype, tuple(t.shape)) if torch.is_tensor(t) else t}")
+                else:
+                    new[name] = t.detach().to(p.device, copy=True).contiguous()
+            fresh[p] = new
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        for group in self.param_groups:
+            group["capturable"] = True
+        self._slots = {}
+        for p, new in fresh.items():
+            self.state[p] = new
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "state_bits": self.state_bits}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._slots = {}

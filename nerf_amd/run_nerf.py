@@ -188,15 +188,22 @@ def create_nerf(args):
         embeddirs_fn, input_ch_views = get_embedder(args.multires_views, args.i_embed)
     output_ch = 5 if args.N_importance > 0 else 4
     skips = [4]
+    # (options upstream lacks; a caller's own argument object may not have them)
+    layer_norm = getattr(args, 'layer_norm', False)
     model = NeRF(D=args.netdepth, W=args.netwidth, input_ch=input_ch, output_ch=output_ch, skips=skips,
-                 input_ch_views=input_ch_views, use_viewdirs=args.use_viewdirs).to(dev)
+                 input_ch_views=input_ch_views, use_viewdirs=args.use_viewdirs, layer_norm=layer_norm).to(dev)
     grad_vars = list(model.parameters())
 
     model_fine = None
     if args.N_importance > 0:
         model_fine = NeRF(D=args.netdepth_fine, W=args.netwidth_fine, input_ch=input_ch, output_ch=output_ch,
-                          skips=skips, input_ch_views=input_ch_views, use_viewdirs=args.use_viewdirs).to(dev)
+                          skips=skips, input_ch_views=input_ch_views, use_viewdirs=args.use_viewdirs,
+                          layer_norm=layer_norm).to(dev)
         grad_vars += list(model_fine.parameters())
+
+    for net in (model, model_fine):
+        if net is not None:
+            net.layer_dtype = getattr(args, 'layer_dtype', 'f32')
 
     network_query_fn = lambda inputs, viewdirs, network_fn: run_network(inputs, viewdirs, network_fn,
                                                                         embed_fn=embed_fn,
@@ -212,8 +219,12 @@ def create_nerf(args):
     # (torch.optim.Adam with the same state and checkpoint format; the parameters of each network lie back to back, and so
     # do their gradients, so a step is one launch of the library's Adam kernel over both networks; step counters and,
     # if it is made a tensor, the learning rate live on the device, so the optimiser can be recorded into a HIP graph)
-    from .optim import FlatAdam
-    optimizer = FlatAdam(params=grad_vars, lr=args.lrate, betas=(0.9, 0.999))
+    from .optim import AdamW, FlatAdam
+    if getattr(args, 'optimizer', 'adam') == 'adamw':
+        optimizer = AdamW(params=grad_vars, lr=args.lrate, betas=(0.9, 0.999), weight_decay=args.weight_decay,
+                          state_bits=args.state_bits)
+    else:
+        optimizer = FlatAdam(params=grad_vars, lr=args.lrate, betas=(0.9, 0.999))
 
     start = 0
     basedir = args.basedir
@@ -387,6 +398,13 @@ def config_parser():
     parser.add_argument("--netwidth", type=int, default=256, help='channels per layer')
     parser.add_argument("--netdepth_fine", type=int, default=8, help='layers in fine network')
     parser.add_argument("--netwidth_fine", type=int, default=256, help='channels per layer in fine network')
+    # (not upstream's: wide and deep networks)
+    parser.add_argument("--layer_norm", action='store_true', help='layer norm behind the ReLU of every hidden layer of the point branch')
+    parser.add_argument("--layer_dtype", type=str, default='f32', choices=['f32', 'fp8'],
+                        help='products of the hidden layers; fp8: both operands in 8 bits, a scale per row and 128 values')
+    parser.add_argument("--optimizer", type=str, default='adam', choices=['adam', 'adamw'], help='update rule')
+    parser.add_argument("--weight_decay", type=float, default=1e-2, help='decoupled weight decay (adamw)')
+    parser.add_argument("--state_bits", type=int, default=32, choices=[32, 8], help='bits of each of the optimiser states (adamw)')
     parser.add_argument("--N_rand", type=int, default=32 * 32 * 4, help='batch size (number of random rays per gradient step)')
     parser.add_argument("--lrate", type=float, default=5e-4, help='learning rate')
     parser.add_argument("--lrate_decay", type=int, default=250, help='exponential learning rate decay (in 1000 steps)')

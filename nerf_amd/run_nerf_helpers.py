@@ -120,9 +120,14 @@ class NeRF(nn.Module):
     The kernel exists for the architecture every upstream config uses: D=8, W=256, skips=[4],
     input_ch=63 (L=10), input_ch_views=27 (L=4) or no view branch.  Any other shape (other --netdepth /
     --netwidth / --multires, --i_embed -1) runs layer by layer through the library's generic matrix kernel
-    (ops.linear) -- same results, autograd included (inputs too), none of the fusion."""
+    (ops.linear) -- same results, autograd included (inputs too), none of the fusion.
 
-    def __init__(self, D=8, W=256, input_ch=3, input_ch_views=3, output_ch=4, skips=[4], use_viewdirs=False):
+    Two options that upstream lacks, for wide and deep networks, take the same layer-by-layer route: layer_norm=True puts
+    a layer norm (ops.layer_norm) behind the ReLU of every pts_linears layer, and layer_dtype = 'fp8' runs the W-wide products in
+    8 bits (ops.linear_fp8)."""
+
+    def __init__(self, D=8, W=256, input_ch=3, input_ch_views=3, output_ch=4, skips=[4], use_viewdirs=False,
+                 layer_norm=False):
         super(NeRF, self).__init__()
         self.D = D
         self.W = W
@@ -142,6 +147,11 @@ class NeRF(nn.Module):
             self.rgb_linear = nn.Linear(W // 2, 3)
         else:
             self.output_linear = nn.Linear(W, output_ch)
+        self.pts_norms = nn.ModuleList([nn.LayerNorm(W) for _ in range(D)]) if layer_norm else None
+        # Products of the layer-by-layer route: 'f32' (default), or 'fp8' = both operands in 8 bits with a power-of-two scale per
+        # row and 128 values, for the layers that read a hidden vector and are W wide (pts_linears behind the first, feature_linear);
+        # the layers at the network's two ends, which are narrow, stay in fp32
+        self.layer_dtype = 'f32'
         self._pack_key = None
         self._pack = None
         self._pack16 = None
@@ -178,7 +188,9 @@ class NeRF(nn.Module):
     # -- kernel plumbing ---------------------------------------------------------------------------
     def fused_arch(self) -> bool:
         """Whether the hand-written kernels cover this module's shape."""
-        return (self.D == 8 and self.W == 256 and list(self.skips) == [4] and self.input_ch == 63
+        if self.layer_dtype not in ('f32', 'fp8'):
+            raise ValueError(f"NeRF.layer_dtype: {self.layer_dtype!r} is neither 'f32' nor 'fp8'")
+        return (self.pts_norms is None and self.layer_dtype == 'f32' and self.D == 8 and self.W == 256 and list(self.skips) == [4] and self.input_ch == 63
                 and ((self.use_viewdirs and self.input_ch_views == 27) or
                      (not self.use_viewdirs and self.input_ch_views == 0 and 1 <= self.output_ch <= 8)))
 
@@ -358,16 +370,23 @@ class NeRF(nn.Module):
         concatenations and splits are PyTorch views and copies."""
         def lin(layer, h, relu):
             return ops.linear(h, layer.weight, layer.bias, relu)
+        wide = lin
+        if self.layer_dtype == 'fp8':
+            def wide(layer, h, relu):
+                return ops.linear_fp8(h, layer.weight, layer.bias, relu)
         pts, views = torch.split(x, [self.input_ch, self.input_ch_views], dim=-1)
         h = pts
         for i, layer in enumerate(self.pts_linears):
-            h = lin(layer, h, True)
+            h = (wide if i > 0 else lin)(layer, h, True)
+            if self.pts_norms is not None:
+                norm = self.pts_norms[i]
+                h = ops.layer_norm(h, norm.weight, norm.bias, norm.eps)
             if i in self.skips:
                 h = torch.cat([pts, h], -1)
         if not self.use_viewdirs:
             return lin(self.output_linear, h, False)
         alpha = lin(self.alpha_linear, h, False)
-        h = torch.cat([lin(self.feature_linear, h, False), views], -1)
+        h = torch.cat([wide(self.feature_linear, h, False), views], -1)
         for layer in self.views_linears:
             h = lin(layer, h, True)
         return torch.cat([lin(self.rgb_linear, h, False), alpha], -1)

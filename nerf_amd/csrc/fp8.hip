@@ -172,6 +172,7 @@ struct Product {
     int bias_f32, relu;
     void* c;
     int64_t ldc;
+    int wide;                 // rows of c start at multiples of 16 bytes
 };
 
 template <typename T>
@@ -252,13 +253,270 @@ __global__ void __launch_bounds__(64 * FEW_WAVES) k_product_few(Product p) {
     }
 }
 
+// ---- tiles --------------------------------------------------------------------------------------------------------------------
+// A workgroup of four waves owns a BM x BN tile of C, a wave a quarter of it in 32 x 32 pieces.  Per 128 of k, (BM + BN) rows of 128 bytes
+// go from memory straight into LDS (buffer_load ... lds, 16 bytes a lane; rows behind the matrix's last read as 0), one step ahead of
+// the multiplication, into the other of two images.  The 16-byte pieces of a row are stored in the order piece ^ (row & 7), so that eight
+// neighbouring rows' reads of one piece cover all banks.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mul32_fp8(i32x8 a, int sa, i32x8 b, int sb, f32x16 acc) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc, 0, 0, 0, sa, 0, sb);
+}
+
+template <int ROWS>
+struct Stage {      // one operand's rows on their way into LDS
+    __amdgpu_buffer_rsrc_t rsrc;
+    int voffset;
+    int ldk;
+    __device__ __forceinline__ Stage(const uint8_t* base, int64_t row0, int64_t rows, int64_t ldk_) : ldk((int)ldk_) {
+        const int64_t left = rows - row0 < ROWS ? rows - row0 : ROWS;
+        rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(base + row0 * ldk_), 0, (int)(unsigned)(left * ldk_), 0x00027000);
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int r = lane >> 3;      // of the eight rows of an instruction
+        voffset = (8 * wave + r) * ldk + ((lane & 7) ^ r) * 16;
+    }
+    // rows 8 wave + 32 i .. + 7 of block kb into their place in `image`
+    __device__ __forceinline__ void issue(int kb, uint8_t* image) const {
+        const int wave = threadIdx.x >> 6;
+#pragma unroll
+        for (int i = 0; i < ROWS / 32; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(image + (8 * wave + 32 * i) * KB), 16, voffset,
+                                                     32 * i * ldk + kb * KB, 0, 0);
+    }
+};
+
+__device__ __forceinline__ i32x8 piece32(const uint8_t* image, int row, int p0) {      // pieces p0 and p0 + 1 of a row
+    const uint4 x = *reinterpret_cast<const uint4*>(image + row * KB + ((p0 ^ (row & 7)) << 4));
+    const uint4 y = *reinterpret_cast<const uint4*>(image + row * KB + (((p0 + 1) ^ (row & 7)) << 4));
+    i32x8 r;
+    r[0] = x.x; r[1] = x.y; r[2] = x.z; r[3] = x.w; r[4] = y.x; r[5] = y.y; r[6] = y.z; r[7] = y.w;
+    return r;
+}
+
+// 32 rows x COLS columns of a wave's LDS image to out[row][col], each lane 16 bytes of a row at a time
+template <typename T, int COLS, int LD>
+__device__ __forceinline__ void emit(const float* image, const Product& p, int64_t row0, int64_t col0, T* out, int64_t ldo, bool wide, bool last) {
+    constexpr int VEC = 16 / sizeof(T), GROUPS = COLS / VEC, ROWS = 64 / GROUPS;
+    const int lane = threadIdx.x & 63;
+    const int c = (lane % GROUPS) * VEC, rl = lane / GROUPS;
+    const int64_t col = col0 + c;
+    if (col >= p.n) return;
+    const bool whole = wide && col + VEC <= p.n;
+    float bias[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+        bias[e] = last && p.bias && col + e < p.n ? (p.bias_f32 ? ((const float*)p.bias)[col + e] : (float)((const T*)p.bias)[col + e]) : 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < 32 / ROWS; ++i) {
+        const int64_t row = row0 + i * ROWS + rl;
+        if (row >= p.m) break;
+        float v[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(image + (i * ROWS + rl) * LD + c + e);
+            v[e] = q.x; v[e + 1] = q.y; v[e + 2] = q.z; v[e + 3] = q.w;
+        }
+        if (last) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                v[e] += bias[e];
+                if (p.relu) v[e] = v[e] > 0.0f ? v[e] : (v[e] != v[e] ? v[e] : 0.0f);      // keeps a NaN
+            }
+        }
+        T* dst = out + row * ldo + col;
+        if (whole) {
+            store_vec<T, VEC>(dst, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (col + e < p.n) dst[e] = (T)v[e];
+        }
+    }
+}
+
+template <typename T, int BM, int BN>
+__global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, int tiles_n, int blocks_per_slice, float* __restrict__ partial) {
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int MT = BM / 64, NT = BN / 64;      // 32 x 32 pieces of a wave
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, g = lane >> 5;
+    // neighbouring tiles on one XCD (workgroups go to the eight XCDs in turn), in bands of four rows of tiles
+    int id = blockIdx.x;
+    const int total = tiles_m * tiles_n;
+    {
+        const int per = total / 8, extra = total % 8, x = id & 7, y = id >> 3;
+        id = x * per + (x < extra ? x : extra) + y;
+    }
+    constexpr int BAND = 4;
+    const int band = id / (BAND * tiles_n), in_band = id - band * BAND * tiles_n;
+    const int band_rows = tiles_m - band * BAND < BAND ? tiles_m - band * BAND : BAND;
+    const int64_t i0 = (int64_t)(band * BAND + in_band % band_rows) * BM, j0 = (int64_t)(in_band / band_rows) * BN;
+    const int kb0 = blockIdx.z * blocks_per_slice;
+    const int kb1 = kb0 + blocks_per_slice < p.blocks ? kb0 + blocks_per_slice : p.blocks;
+
+    const Stage<BM> sa(p.a, i0, p.m, p.ldk);
+    const Stage<BN> sb(p.b, j0, p.n, p.ldk);
+    const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
+    const uint8_t *sap[MT], *sbp[NT];      // scales, four blocks to a word
+#pragma unroll
+    for (int t = 0; t < MT; ++t) { const int64_t i = i0 + wm + 32 * t + r; sap[t] = p.sa + (i < p.m ? i : p.m - 1) * p.lds; }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) { const int64_t j = j0 + wn + 32 * t + r; sbp[t] = p.sb + (j < p.n ? j : p.n - 1) * p.lds; }
+
+    f32x16 acc[MT][NT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[t][u][e] = 0.0f;
+
+    auto words = [&](int kb, unsigned (&wa)[MT], unsigned (&wb)[NT]) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) wa[t] = *reinterpret_cast<const unsigned*>(sap[t] + (kb & ~3));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) wb[t] = *reinterpret_cast<const unsigned*>(sbp[t] + (kb & ~3));
+    };
+    constexpr int IMAGE = (BM + BN) * KB;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    unsigned wa[MT], wb[NT], na[MT], nb[NT];
+    int cur = 0;
+    if (kb0 < kb1) {
+        sa.issue(kb0, lds);
+        sb.issue(kb0, lds + BM * KB);
+        words(kb0, na, nb);
+    }
+    for (int kb = kb0; kb < kb1; ++kb) {
+        // this wave's rows are in LDS, then everyone's; and everyone is done with the other image
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        asm volatile("s_barrier" ::: "memory");
+        const int sh = 8 * (kb & 3);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) wa[t] = na[t] >> sh;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) wb[t] = nb[t] >> sh;
+        const uint8_t *am = lds + cur, *bm = am + BM * KB;
+        cur = IMAGE - cur;
+        if (kb + 1 < kb1) {
+            sa.issue(kb + 1, lds + cur);
+            sb.issue(kb + 1, lds + cur + BM * KB);
+            words(kb + 1, na, nb);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            i32x8 af[MT], bf[NT];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) af[t] = piece32(am, wm + 32 * t + r, 4 * h + 2 * g);
+#pragma unroll
+            for (int u = 0; u < NT; ++u) bf[u] = piece32(bm, wn + 32 * u + r, 4 * h + 2 * g);
+            if constexpr (!F32) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int u = 0; u < NT; ++u) acc[t][u] = mul32_fp8(af[t], (int)wa[t], bf[u], (int)wb[u], acc[t][u]);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    bf16x8 ad[MT], bd[NT];
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) ad[t] = decode8(af[t][2 * q], af[t][2 * q + 1], __uint_as_float((wa[t] & 255u) << 23));
+#pragma unroll
+                    for (int u = 0; u < NT; ++u) bd[u] = decode8(bf[u][2 * q], bf[u][2 * q + 1], __uint_as_float((wb[u] & 255u) << 23));
+#pragma unroll
+                    for (int t = 0; t < MT; ++t)
+#pragma unroll
+                        for (int u = 0; u < NT; ++u) acc[t][u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ad[t], bd[u], acc[t][u], 0, 0, 0);
+                }
+            }
+        }
+    }
+    // out through LDS, 32 rows of the wave's columns at a time, so that a store is 16 bytes of a row (or fp32 partial sums likewise)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    asm volatile("s_barrier" ::: "memory");
+    constexpr int COLS = 32 * NT, LD = COLS + 4;
+    static_assert(4 * 32 * LD * sizeof(float) <= 2 * IMAGE, "the bands of four waves lie in the images");
+    float* band_image = reinterpret_cast<float*>(lds) + wave * 32 * LD;
+    const bool sums = partial != nullptr;
+    const int64_t col0 = j0 + wn;
+    float* part = sums ? partial + (int64_t)blockIdx.z * p.m * p.n : nullptr;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) band_image[((e & 3) + 8 * (e >> 2) + 4 * g) * LD + 32 * u + r] = acc[t][u][e];
+        const int64_t row0 = i0 + wm + 32 * t;
+        if (sums) emit<float, COLS, LD>(band_image, p, row0, col0, part, p.n, (p.n & 3) == 0, false);
+        else emit<T, COLS, LD>(band_image, p, row0, col0, (T*)p.c, p.ldc, p.wide != 0, true);
+    }
+}
+
+// c = act(sum over the slices of k, in their order, + bias)
 template <typename T>
-int product(const Product& p, hipStream_t stream) {
-    constexpr int MT = 4;
-    const int64_t gx = (p.n + 15) / 16, gy = (p.m + 16 * MT - 1) / (16 * MT);
-    if (gx > 0x7fffff || gy > 65535) return fail(NERF_E_ARG, "nerf_fp8_matmul: %lld x %lld is more than one launch covers", (long long)p.m, (long long)p.n);
-    hipLaunchKernelGGL((k_product_few<T, MT>), dim3((unsigned)gx, (unsigned)gy), dim3(64 * FEW_WAVES), 0, stream, p);
-    return launched("nerf_fp8_matmul");
+__global__ void __launch_bounds__(256) k_product_join(Product p, int slices, const float* __restrict__ partial) {
+    const int64_t size = p.m * p.n;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
+        float s = 0.0f;
+        for (int z = 0; z < slices; ++z) s += partial[z * size + i];
+        const int64_t row = i / p.n, col = i - row * p.n;
+        ((T*)p.c)[row * p.ldc + col] = (T)finish<T>(s, p, col);
+    }
+}
+
+// How a product is cut, from its sizes alone.
+struct Plan {
+    int tile;           // 0: few rows; else the tile's edge
+    int slices;         // of k
+    int blocks_per_slice;
+};
+Plan plan_of(int64_t m, int64_t n, int64_t k, int type) {
+    const int64_t blocks = blocks_of(k);
+    if (m <= 64 || k > (1 << 22)) return {0, 1, (int)blocks};
+    auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
+    const int cus = 256;
+    const int tile = type != NERF_F32 && tiles(256) >= cus ? 256 : 128;
+    int64_t slices = 1;
+    const int64_t count = tiles(tile);
+    if (count < 2 * cus) slices = (2 * cus + count - 1) / count;
+    if (slices > blocks / 4) slices = blocks / 4;
+    if (slices < 1) slices = 1;
+    const int64_t per = (blocks + slices - 1) / slices;
+    return {tile, (int)((blocks + per - 1) / per), (int)per};
+}
+
+template <typename T>
+int product(const Product& p, int64_t k, int type, float* ws, hipStream_t stream) {
+    const Plan plan = plan_of(p.m, p.n, k, type);
+    if (plan.tile == 0) {
+        constexpr int MT = 4;
+        const int64_t gx = (p.n + 15) / 16, gy = (p.m + 16 * MT - 1) / (16 * MT);
+        if (gx > 0x7fffff || gy > 65535) return fail(NERF_E_ARG, "nerf_fp8_matmul: %lld x %lld is more than one launch covers", (long long)p.m, (long long)p.n);
+        hipLaunchKernelGGL((k_product_few<T, MT>), dim3((unsigned)gx, (unsigned)gy), dim3(64 * FEW_WAVES), 0, stream, p);
+        return launched("nerf_fp8_matmul");
+    }
+    const int64_t tm = (p.m + plan.tile - 1) / plan.tile, tn = (p.n + plan.tile - 1) / plan.tile;
+    if (tm * tn > 0xffffff) return fail(NERF_E_ARG, "nerf_fp8_matmul: %lld x %lld is more than one launch covers", (long long)p.m, (long long)p.n);
+    const dim3 grid((unsigned)(tm * tn), 1, (unsigned)plan.slices);
+    float* part = plan.slices > 1 ? ws : nullptr;
+    if (plan.slices > 1 && !ws) return fail(NERF_E_ARG, "nerf_fp8_matmul: null workspace");
+#define GO(E)                                                                                                                        \
+    do {                                                                                                                             \
+        constexpr size_t bytes = 2 * (E + E) * KB;                                                                                   \
+        const hipError_t e = lds_limit_once((const void*)&k_product_tile<T, E, E>, bytes);                                           \
+        if (e != hipSuccess) return fail(NERF_E_LAUNCH, "nerf_fp8_matmul: %s", hipGetErrorString(e));                                \
+        hipLaunchKernelGGL((k_product_tile<T, E, E>), grid, dim3(256), bytes, stream, p, (int)tm, (int)tn, plan.blocks_per_slice, part); \
+    } while (0)
+    if constexpr (sizeof(T) == 2) {
+        if (plan.tile == 256) GO(256); else GO(128);
+    } else {
+        GO(128);
+    }
+#undef GO
+    const int rc = launched("nerf_fp8_matmul");
+    if (rc || !part) return rc;
+    const int64_t wgs = (p.m * p.n + 255) / 256;
+    hipLaunchKernelGGL((k_product_join<T>), dim3((unsigned)(wgs < 4096 ? wgs : 4096)), dim3(256), 0, stream, p, plan.slices, part);
+    return launched("nerf_fp8_matmul (join)");
 }
 
 template <typename T>
@@ -328,17 +586,18 @@ int nerf_fp8_matmul(int64_t m, int64_t n, int64_t k, const uint8_t* a, const uin
     NERF_REQUIRE(((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0 &&
                  ((reinterpret_cast<uintptr_t>(a_scales) | reinterpret_cast<uintptr_t>(b_scales)) & 3) == 0,
                  "nerf_fp8_matmul: codes start at a multiple of 16 bytes, scales of 4");
-    (void)workspace;
-    Product p{a, b, a_scales, b_scales, m, n, code_stride(k), scale_stride(k), (int)blocks_of(k), bias, bias_type == NERF_F32, relu, c, ldc};
+    Product p{a, b, a_scales, b_scales, m, n, code_stride(k), scale_stride(k), (int)blocks_of(k), bias, bias_type == NERF_F32, relu, c, ldc,
+              ((reinterpret_cast<uintptr_t>(c) | (uintptr_t)(ldc * elem_size(type))) & 15) == 0};
     hipStream_t stream = as_stream(stream_);
-    if (type == NERF_F32) return product<float>(p, stream);
-    if (type == NERF_BF16) return product<bf16_t>(p, stream);
-    return product<f16_t>(p, stream);
+    if (type == NERF_F32) return product<float>(p, k, type, workspace, stream);
+    if (type == NERF_BF16) return product<bf16_t>(p, k, type, workspace, stream);
+    return product<f16_t>(p, k, type, workspace, stream);
 }
 
 int64_t nerf_fp8_matmul_workspace_floats(int64_t m, int64_t n, int64_t k, int type) {
-    (void)m; (void)n; (void)k; (void)type;
-    return 0;
+    if (m < 1 || n < 1 || k < 1) return 0;
+    const Plan plan = plan_of(m, n, k, type);
+    return plan.slices > 1 ? plan.slices * m * n : 0;
 }
 
 }  // extern "C"

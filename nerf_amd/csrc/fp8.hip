@@ -254,44 +254,52 @@ __global__ void __launch_bounds__(64 * FEW_WAVES) k_product_few(Product p) {
 }
 
 // ---- tiles --------------------------------------------------------------------------------------------------------------------
-// A workgroup of four waves owns a BM x BN tile of C, a wave a quarter of it in 32 x 32 pieces.  Per 128 of k, (BM + BN) rows of 128 bytes
-// go from memory straight into LDS (buffer_load ... lds, 16 bytes a lane; rows behind the matrix's last read as 0), one step ahead of
-// the multiplication, into the other of two images.  The 16-byte pieces of a row are stored in the order piece ^ (row & 7), so that eight
-// neighbouring rows' reads of one piece cover all banks.
+// A workgroup of four waves owns a BM x BN tile of C, a wave a quarter of it in 32 x 32 pieces.  k advances in steps of 64, half a
+// block.  Per step (BM + BN) rows of 64 bytes go from memory straight into LDS (global_load_lds, 16 bytes a lane), into one of four
+// images in turn; while step s multiplies out of registers, the fragments of step s + 1 are read from their image into a second
+// set of registers and the rows of step s + 3 are under way, so that neither latency is waited for: one barrier per step.  The 16-byte
+// pieces of a row are stored in the order piece ^ (row / 2 & 3), so that eight neighbouring rows' reads of one piece cover all banks.
+constexpr int KH = 64;        // bytes of a row in an image
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ f32x16 mul32_fp8(i32x8 a, int sa, i32x8 b, int sb, f32x16 acc) {
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc, 0, 0, 0, sa, 0, sb);
 }
 
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }      // in a scalar register
+
 template <int ROWS>
 struct Stage {      // one operand's rows on their way into LDS
-    __amdgpu_buffer_rsrc_t rsrc;
-    int voffset;
-    int ldk;
-    __device__ __forceinline__ Stage(const uint8_t* base, int64_t row0, int64_t rows, int64_t ldk_) : ldk((int)ldk_) {
-        const int64_t left = rows - row0 < ROWS ? rows - row0 : ROWS;
-        rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(base + row0 * ldk_), 0, (int)(unsigned)(left * ldk_), 0x00027000);
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const int r = lane >> 3;      // of the eight rows of an instruction
-        voffset = (8 * wave + r) * ldk + ((lane & 7) ^ r) * 16;
-    }
-    // rows 8 wave + 32 i .. + 7 of block kb into their place in `image`
-    __device__ __forceinline__ void issue(int kb, uint8_t* image) const {
-        const int wave = threadIdx.x >> 6;
+    static constexpr int N = ROWS / 64;      // instructions of a wave per step, sixteen rows each
+    const uint8_t* base;
+    unsigned offset[N];      // of this lane's 16 bytes; rows behind the last stand for the last
+    __device__ __forceinline__ Stage(const uint8_t* p, int64_t row0, int64_t rows, int64_t ldk) : base(p + row0 * ldk) {
+        const int lane = threadIdx.x & 63, wave = wave_id();
+        const int last = (int)(rows - row0 < ROWS ? rows - row0 : ROWS) - 1;
+        const int r = lane >> 2;
 #pragma unroll
-        for (int i = 0; i < ROWS / 32; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(image + (8 * wave + 32 * i) * KB), 16, voffset,
-                                                     32 * i * ldk + kb * KB, 0, 0);
+        for (int i = 0; i < N; ++i) {
+            const int row = 16 * (wave + 4 * i) + r;
+            offset[i] = (unsigned)(row < last ? row : last) * (unsigned)ldk + (((lane & 3) ^ (r >> 1 & 3)) << 4);
+        }
+    }
+    __device__ __forceinline__ void issue(int step, uint8_t* image) const {
+        const int wave = wave_id();
+        const uint8_t* src = base + (int64_t)step * KH;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + offset[i]),
+                                             (__attribute__((address_space(3))) void*)(image + 16 * (wave + 4 * i) * KH), 16, 0, 0);
     }
 };
 
-__device__ __forceinline__ i32x8 piece32(const uint8_t* image, int row, int p0) {      // pieces p0 and p0 + 1 of a row
-    const uint4 x = *reinterpret_cast<const uint4*>(image + row * KB + ((p0 ^ (row & 7)) << 4));
-    const uint4 y = *reinterpret_cast<const uint4*>(image + row * KB + (((p0 + 1) ^ (row & 7)) << 4));
-    i32x8 r;
-    r[0] = x.x; r[1] = x.y; r[2] = x.z; r[3] = x.w; r[4] = y.x; r[5] = y.y; r[6] = y.z; r[7] = y.w;
-    return r;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+// 32 of the 64 bytes of a row: pieces 2 g and 2 g + 1
+__device__ __forceinline__ i32x8 piece32(const uint8_t* image, int row, int g) {
+    const int sw = row >> 1 & 3;
+    const i32x4 x = *reinterpret_cast<const i32x4*>(image + row * KH + (((2 * g) ^ sw) << 4));
+    const i32x4 y = *reinterpret_cast<const i32x4*>(image + row * KH + (((2 * g + 1) ^ sw) << 4));
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 // 32 rows x COLS columns of a wave's LDS image to out[row][col], each lane 16 bytes of a row at a time
@@ -339,7 +347,7 @@ template <typename T, int BM, int BN>
 __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, int tiles_n, int blocks_per_slice, float* __restrict__ partial) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int MT = BM / 64, NT = BN / 64;      // 32 x 32 pieces of a wave
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, g = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = wave_id(), r = lane & 31, g = lane >> 5;
     // neighbouring tiles on one XCD (workgroups go to the eight XCDs in turn), in bands of four rows of tiles
     int id = blockIdx.x;
     const int total = tiles_m * tiles_n;
@@ -357,12 +365,6 @@ __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, in
     const Stage<BM> sa(p.a, i0, p.m, p.ldk);
     const Stage<BN> sb(p.b, j0, p.n, p.ldk);
     const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
-    const uint8_t *sap[MT], *sbp[NT];      // scales, four blocks to a word
-#pragma unroll
-    for (int t = 0; t < MT; ++t) { const int64_t i = i0 + wm + 32 * t + r; sap[t] = p.sa + (i < p.m ? i : p.m - 1) * p.lds; }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) { const int64_t j = j0 + wn + 32 * t + r; sbp[t] = p.sb + (j < p.n ? j : p.n - 1) * p.lds; }
-
     f32x16 acc[MT][NT];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
@@ -371,70 +373,124 @@ __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, in
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[t][u][e] = 0.0f;
 
-    auto words = [&](int kb, unsigned (&wa)[MT], unsigned (&wb)[NT]) {
+    constexpr int IMAGE = (BM + BN) * KH, WORDS = (BM + BN) * 4;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];      // four images, two sets of scale words
+    // the scales of four blocks are a word per row; a set of words comes along with the first image that needs it
+    constexpr int SROWS = (BM + BN) / 4;      // rows of a wave
+    const uint8_t* srow[SROWS / 64];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) wa[t] = *reinterpret_cast<const unsigned*>(sap[t] + (kb & ~3));
-#pragma unroll
-        for (int t = 0; t < NT; ++t) wb[t] = *reinterpret_cast<const unsigned*>(sbp[t] + (kb & ~3));
-    };
-    constexpr int IMAGE = (BM + BN) * KB;
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    unsigned wa[MT], wb[NT], na[MT], nb[NT];
-    int cur = 0;
-    if (kb0 < kb1) {
-        sa.issue(kb0, lds);
-        sb.issue(kb0, lds + BM * KB);
-        words(kb0, na, nb);
+    for (int i = 0; i < SROWS / 64; ++i) {
+        const int row = SROWS * wave + 64 * i + lane;      // A's rows, then B's
+        if (SROWS * wave + 64 * i < BM) srow[i] = p.sa + (i0 + row < p.m ? i0 + row : p.m - 1) * p.lds;
+        else srow[i] = p.sb + (j0 + row - BM < p.n ? j0 + row - BM : p.n - 1) * p.lds;
     }
-    for (int kb = kb0; kb < kb1; ++kb) {
-        // this wave's rows are in LDS, then everyone's; and everyone is done with the other image
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        asm volatile("s_barrier" ::: "memory");
+    uint8_t* const words = lds + 4 * IMAGE;
+    auto issue_words = [&](int group) {
+#pragma unroll
+        for (int i = 0; i < SROWS / 64; ++i)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(srow[i] + 4 * (int64_t)group),
+                                             (__attribute__((address_space(3))) void*)(words + (group & 1) * WORDS + (SROWS * wave + 64 * i) * 4), 4, 0, 0);
+    };
+    const int s0 = 2 * kb0, s1 = 2 * kb1;
+    // (no branches: behind the last step its rows come once more, into an image that nobody reads any longer)
+    auto issue = [&](int step, int place) {
+        uint8_t* image = lds + (place & 3) * IMAGE;
+        sa.issue(step, image);
+        sb.issue(step, image + BM * KH);
+    };
+    auto clamp = [&](int step) { return step < s1 ? step : s1 - 1; };
+    constexpr int PER_STEP = Stage<BM>::N + Stage<BN>::N;      // this wave's row instructions of a step
+    i32x8 af[2][MT], bf[2][NT];
+    unsigned wa[MT], wb[NT], na[MT], nb[NT];
+    auto fetch = [&](int step, i32x8 (&a)[MT], i32x8 (&b)[NT]) {
+        const uint8_t *am = lds + (step & 3) * IMAGE, *bm = am + BM * KH;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) a[t] = piece32(am, wm + 32 * t + r, g);
+#pragma unroll
+        for (int u = 0; u < NT; ++u) b[u] = piece32(bm, wn + 32 * u + r, g);
+    };
+    auto fetch_words = [&](int kb, unsigned (&a)[MT], unsigned (&b)[NT]) {
+        const unsigned* w = reinterpret_cast<const unsigned*>(words + ((kb >> 2) & 1) * WORDS);
         const int sh = 8 * (kb & 3);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) wa[t] = na[t] >> sh;
+        for (int t = 0; t < MT; ++t) a[t] = w[wm + 32 * t + r] >> sh;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) wb[t] = nb[t] >> sh;
-        const uint8_t *am = lds + cur, *bm = am + BM * KB;
-        cur = IMAGE - cur;
-        if (kb + 1 < kb1) {
-            sa.issue(kb + 1, lds + cur);
-            sb.issue(kb + 1, lds + cur + BM * KB);
-            words(kb + 1, na, nb);
+        for (int u = 0; u < NT; ++u) b[u] = w[BM + wn + 32 * u + r] >> sh;
+    };
+    // the rows of the step after this one are in LDS: those of the step behind it may still be out, and the scale words among them;
+    // and every wave is done with the image that is overwritten next
+    auto landed = [&] {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER_STEP) : "memory");
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // one step's reads and requests spread over its multiplications
+    auto spread = [&] {
+        if constexpr (!F32) {
+#pragma unroll
+            for (int i = 0; i < MT * NT; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);      // a matrix instruction
+                __builtin_amdgcn_sched_group_barrier(0x100, (2 * (MT + NT) + MT * NT - 1) / (MT * NT), 0);      // reads of LDS
+                __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);      // a request
+            }
         }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto multiply = [&](const i32x8 (&a)[MT], const i32x8 (&b)[NT]) {
+        if constexpr (!F32) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            i32x8 af[MT], bf[NT];
+            for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int t = 0; t < MT; ++t) af[t] = piece32(am, wm + 32 * t + r, 4 * h + 2 * g);
+                for (int u = 0; u < NT; ++u) acc[t][u] = mul32_fp8(a[t], (int)wa[t], b[u], (int)wb[u], acc[t][u]);
+        } else {
 #pragma unroll
-            for (int u = 0; u < NT; ++u) bf[u] = piece32(bm, wn + 32 * u + r, 4 * h + 2 * g);
-            if constexpr (!F32) {
+            for (int q = 0; q < 4; ++q) {
+                bf16x8 ad[MT], bd[NT];
+#pragma unroll
+                for (int t = 0; t < MT; ++t) ad[t] = decode8(a[t][2 * q], a[t][2 * q + 1], __uint_as_float((wa[t] & 255u) << 23));
+#pragma unroll
+                for (int u = 0; u < NT; ++u) bd[u] = decode8(b[u][2 * q], b[u][2 * q + 1], __uint_as_float((wb[u] & 255u) << 23));
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
 #pragma unroll
-                    for (int u = 0; u < NT; ++u) acc[t][u] = mul32_fp8(af[t], (int)wa[t], bf[u], (int)wb[u], acc[t][u]);
-            } else {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    bf16x8 ad[MT], bd[NT];
-#pragma unroll
-                    for (int t = 0; t < MT; ++t) ad[t] = decode8(af[t][2 * q], af[t][2 * q + 1], __uint_as_float((wa[t] & 255u) << 23));
-#pragma unroll
-                    for (int u = 0; u < NT; ++u) bd[u] = decode8(bf[u][2 * q], bf[u][2 * q + 1], __uint_as_float((wb[u] & 255u) << 23));
-#pragma unroll
-                    for (int t = 0; t < MT; ++t)
-#pragma unroll
-                        for (int u = 0; u < NT; ++u) acc[t][u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ad[t], bd[u], acc[t][u], 0, 0, 0);
-                }
+                    for (int u = 0; u < NT; ++u) acc[t][u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ad[t], bd[u], acc[t][u], 0, 0, 0);
             }
         }
+    };
+    issue_words(kb0 >> 2);
+    issue(s0, s0);
+    issue(s0 + 1, s0 + 1);
+    issue_words((kb0 + 1 < kb1 ? kb0 + 1 : kb0) >> 2);
+    issue(clamp(s0 + 2), s0 + 2);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER_STEP) : "memory");
+    asm volatile("s_barrier" ::: "memory");
+    fetch(s0, af[0], bf[0]);
+    fetch_words(kb0, na, nb);
+    for (int kb = kb0; kb < kb1; ++kb) {
+        const int s = 2 * kb;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) wa[t] = na[t];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) wb[u] = nb[u];
+        landed();
+        issue(clamp(s + 3), s + 3);
+        fetch(s + 1, af[1], bf[1]);
+        multiply(af[0], bf[0]);
+        spread();
+        landed();
+        issue_words((kb + 2 < kb1 ? kb + 2 : kb1 - 1) >> 2);
+        issue(clamp(s + 4), s + 4);
+        fetch(s + 2, af[0], bf[0]);
+        fetch_words(kb + 1, na, nb);
+        multiply(af[1], bf[1]);
+        spread();
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     // out through LDS, 32 rows of the wave's columns at a time, so that a store is 16 bytes of a row (or fp32 partial sums likewise)
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     asm volatile("s_barrier" ::: "memory");
     constexpr int COLS = 32 * NT, LD = COLS + 4;
-    static_assert(4 * 32 * LD * sizeof(float) <= 2 * IMAGE, "the bands of four waves lie in the images");
+    static_assert(4 * 32 * LD * sizeof(float) <= 4 * IMAGE, "the bands of four waves lie in the images");
     float* band_image = reinterpret_cast<float*>(lds) + wave * 32 * LD;
     const bool sums = partial != nullptr;
     const int64_t col0 = j0 + wn;
@@ -501,7 +557,7 @@ int product(const Product& p, int64_t k, int type, float* ws, hipStream_t stream
     if (plan.slices > 1 && !ws) return fail(NERF_E_ARG, "nerf_fp8_matmul: null workspace");
 #define GO(E)                                                                                                                        \
     do {                                                                                                                             \
-        constexpr size_t bytes = 2 * (E + E) * KB;                                                                                   \
+        constexpr size_t bytes = (E + E) * (4 * KH + 8);                                                                                 \
         const hipError_t e = lds_limit_once((const void*)&k_product_tile<T, E, E>, bytes);                                           \
         if (e != hipSuccess) return fail(NERF_E_LAUNCH, "nerf_fp8_matmul: %s", hipGetErrorString(e));                                \
         hipLaunchKernelGGL((k_product_tile<T, E, E>), grid, dim3(256), bytes, stream, p, (int)tm, (int)tn, plan.blocks_per_slice, part); \

@@ -283,24 +283,26 @@ struct Stage {      // one operand's rows on their way into LDS
             offset[i] = (unsigned)(row < last ? row : last) * (unsigned)ldk + (((lane & 3) ^ (r >> 1 & 3)) << 4);
         }
     }
-    __device__ __forceinline__ void issue(int step, uint8_t* image) const {
-        const int wave = wave_id();
-        const uint8_t* src = base + (int64_t)step * KH;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + offset[i]),
-                                             (__attribute__((address_space(3))) void*)(image + 16 * (wave + 4 * i) * KH), 16, 0, 0);
+    __device__ __forceinline__ void issue(int i, int step, uint8_t* image) const {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + (int64_t)step * KH + offset[i]),
+                                         (__attribute__((address_space(3))) void*)(image + 16 * (wave_id() + 4 * i) * KH), 16, 0, 0);
     }
 };
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-// 32 of the 64 bytes of a row: pieces 2 g and 2 g + 1
-__device__ __forceinline__ i32x8 piece32(const uint8_t* image, int row, int g) {
-    const int sw = row >> 1 & 3;
-    const i32x4 x = *reinterpret_cast<const i32x4*>(image + row * KH + (((2 * g) ^ sw) << 4));
-    const i32x4 y = *reinterpret_cast<const i32x4*>(image + row * KH + (((2 * g + 1) ^ sw) << 4));
-    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-}
+// where a lane's 32 of the 64 bytes of row `row` lie in an image: pieces 2 g and 2 g + 1
+struct Piece {
+    int x, y;
+    __device__ __forceinline__ Piece(int row, int g) {
+        const int sw = row >> 1 & 3;
+        x = row * KH + (((2 * g) ^ sw) << 4);
+        y = row * KH + (((2 * g + 1) ^ sw) << 4);
+    }
+    __device__ __forceinline__ i32x8 read(const uint8_t* image, int t) const {      // of the row 32 t further (the order of its pieces is the same)
+        const i32x4 p = *reinterpret_cast<const i32x4*>(image + x + 32 * t * KH), q = *reinterpret_cast<const i32x4*>(image + y + 32 * t * KH);
+        return __builtin_shufflevector(p, q, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
 
 // 32 rows x COLS columns of a wave's LDS image to out[row][col], each lane 16 bytes of a row at a time
 template <typename T, int COLS, int LD>
@@ -392,30 +394,29 @@ __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, in
                                              (__attribute__((address_space(3))) void*)(words + (group & 1) * WORDS + (SROWS * wave + 64 * i) * 4), 4, 0, 0);
     };
     const int s0 = 2 * kb0, s1 = 2 * kb1;
+    constexpr int NA = Stage<BM>::N, PER_STEP = NA + Stage<BN>::N;      // this wave's row instructions of a step
     // (no branches: behind the last step its rows come once more, into an image that nobody reads any longer)
-    auto issue = [&](int step, int place) {
-        uint8_t* image = lds + (place & 3) * IMAGE;
-        sa.issue(step, image);
-        sb.issue(step, image + BM * KH);
+    auto issue = [&](int i, int step) {
+        uint8_t* image = lds + (step & 3) * IMAGE;
+        const int from = step < s1 ? step : s1 - 1;
+        if (i < NA) sa.issue(i, from, image);
+        else sb.issue(i - NA, from, image + BM * KH);
     };
-    auto clamp = [&](int step) { return step < s1 ? step : s1 - 1; };
-    constexpr int PER_STEP = Stage<BM>::N + Stage<BN>::N;      // this wave's row instructions of a step
+    const Piece pa(wm + r, g), pb(wn + r, g);
     i32x8 af[2][MT], bf[2][NT];
     unsigned wa[MT], wb[NT], na[MT], nb[NT];
-    auto fetch = [&](int step, i32x8 (&a)[MT], i32x8 (&b)[NT]) {
-        const uint8_t *am = lds + (step & 3) * IMAGE, *bm = am + BM * KH;
-#pragma unroll
-        for (int t = 0; t < MT; ++t) a[t] = piece32(am, wm + 32 * t + r, g);
-#pragma unroll
-        for (int u = 0; u < NT; ++u) b[u] = piece32(bm, wn + 32 * u + r, g);
+    auto fetch = [&](int i, int step, i32x8 (&a)[MT], i32x8 (&b)[NT]) {      // piece i of a step's MT + NT
+        const uint8_t* image = lds + (step & 3) * IMAGE;
+        if (i < MT) a[i] = pa.read(image, i);
+        else b[i - MT] = pb.read(image + BM * KH, i - MT);
     };
-    auto fetch_words = [&](int kb, unsigned (&a)[MT], unsigned (&b)[NT]) {
+    auto fetch_words = [&](int kb) {
         const unsigned* w = reinterpret_cast<const unsigned*>(words + ((kb >> 2) & 1) * WORDS);
         const int sh = 8 * (kb & 3);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) a[t] = w[wm + 32 * t + r] >> sh;
+        for (int t = 0; t < MT; ++t) na[t] = w[wm + 32 * t + r] >> sh;
 #pragma unroll
-        for (int u = 0; u < NT; ++u) b[u] = w[BM + wn + 32 * u + r] >> sh;
+        for (int u = 0; u < NT; ++u) nb[u] = w[BM + wn + 32 * u + r] >> sh;
     };
     // the rows of the step after this one are in LDS: those of the step behind it may still be out, and the scale words among them;
     // and every wave is done with the image that is overwritten next
@@ -424,25 +425,26 @@ __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, in
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
-    // one step's reads and requests spread over its multiplications
-    auto spread = [&] {
+    // Step `step` multiplies out of a, b; between its instructions, in this order, the next step's fragments are read into an, bn and
+    // the rows of the step three ahead are asked for.  (One wave per SIMD: what is not placed between matrix instructions, which
+    // take 64 cycles each, is waited for.)
+    auto run = [&](int step, const i32x8 (&a)[MT], const i32x8 (&b)[NT], i32x8 (&an)[MT], i32x8 (&bn)[NT], auto also) {
+        constexpr int M = MT * NT, P = MT + NT;
         if constexpr (!F32) {
 #pragma unroll
-            for (int i = 0; i < MT * NT; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);      // a matrix instruction
-                __builtin_amdgcn_sched_group_barrier(0x100, (2 * (MT + NT) + MT * NT - 1) / (MT * NT), 0);      // reads of LDS
-                __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);      // a request
+            for (int i = 0; i < M; ++i) {
+                acc[i / NT][i % NT] = mul32_fp8(a[i / NT], (int)wa[i / NT], b[i % NT], (int)wb[i % NT], acc[i / NT][i % NT]);
+                if (i < P) fetch(i, step + 1, an, bn);
+                if (i >= M - PER_STEP) issue(i - (M - PER_STEP), step + 3);
+                if (i == (P < M ? P : M - 1)) also();
+                __builtin_amdgcn_sched_barrier(0);
             }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    auto multiply = [&](const i32x8 (&a)[MT], const i32x8 (&b)[NT]) {
-        if constexpr (!F32) {
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int u = 0; u < NT; ++u) acc[t][u] = mul32_fp8(a[t], (int)wa[t], b[u], (int)wb[u], acc[t][u]);
         } else {
+#pragma unroll
+            for (int i = 0; i < P; ++i) fetch(i, step + 1, an, bn);
+#pragma unroll
+            for (int i = 0; i < PER_STEP; ++i) issue(i, step + 3);
+            also();
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 bf16x8 ad[MT], bd[NT];
@@ -455,35 +457,32 @@ __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, in
 #pragma unroll
                     for (int u = 0; u < NT; ++u) acc[t][u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ad[t], bd[u], acc[t][u], 0, 0, 0);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     issue_words(kb0 >> 2);
-    issue(s0, s0);
-    issue(s0 + 1, s0 + 1);
+#pragma unroll
+    for (int i = 0; i < PER_STEP; ++i) issue(i, s0);
+#pragma unroll
+    for (int i = 0; i < PER_STEP; ++i) issue(i, s0 + 1);
     issue_words((kb0 + 1 < kb1 ? kb0 + 1 : kb0) >> 2);
-    issue(clamp(s0 + 2), s0 + 2);
+#pragma unroll
+    for (int i = 0; i < PER_STEP; ++i) issue(i, s0 + 2);
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER_STEP) : "memory");
     asm volatile("s_barrier" ::: "memory");
-    fetch(s0, af[0], bf[0]);
-    fetch_words(kb0, na, nb);
+#pragma unroll
+    for (int i = 0; i < MT + NT; ++i) fetch(i, s0, af[0], bf[0]);
+    fetch_words(kb0);
     for (int kb = kb0; kb < kb1; ++kb) {
-        const int s = 2 * kb;
 #pragma unroll
         for (int t = 0; t < MT; ++t) wa[t] = na[t];
 #pragma unroll
         for (int u = 0; u < NT; ++u) wb[u] = nb[u];
         landed();
-        issue(clamp(s + 3), s + 3);
-        fetch(s + 1, af[1], bf[1]);
-        multiply(af[0], bf[0]);
-        spread();
+        run(2 * kb, af[0], bf[0], af[1], bf[1], [] {});
         landed();
         issue_words((kb + 2 < kb1 ? kb + 2 : kb1 - 1) >> 2);
-        issue(clamp(s + 4), s + 4);
-        fetch(s + 2, af[0], bf[0]);
-        fetch_words(kb + 1, na, nb);
-        multiply(af[1], bf[1]);
-        spread();
+        run(2 * kb + 1, af[1], bf[1], af[0], bf[0], [&] { fetch_words(kb + 1); });
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     // out through LDS, 32 rows of the wave's columns at a time, so that a store is 16 bytes of a row (or fp32 partial sums likewise)

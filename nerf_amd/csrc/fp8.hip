@@ -254,12 +254,13 @@ __global__ void __launch_bounds__(64 * FEW_WAVES) k_product_few(Product p) {
 }
 
 // ---- tiles --------------------------------------------------------------------------------------------------------------------
-// A workgroup of four waves owns a BM x BN tile of C, a wave a quarter of it in 32 x 32 pieces.  k advances in steps of 64, half a
-// block.  Per step (BM + BN) rows of 64 bytes go from memory straight into LDS (global_load_lds, 16 bytes a lane), into one of four
-// images in turn; while step s multiplies out of registers, the fragments of step s + 1 are read from their image into a second
-// set of registers and the rows of step s + 3 are under way, so that neither latency is waited for: one barrier per step.  The 16-byte
-// pieces of a row are stored in the order piece ^ (row / 2 & 3), so that eight neighbouring rows' reads of one piece cover all banks.
-constexpr int KH = 64;        // bytes of a row in an image
+// A workgroup of four waves owns a BM x BN tile of C, a wave a quarter of it in 32 x 32 pieces.  Per block of k, (BM + BN) rows of 128
+// bytes go from memory straight into LDS (global_load_lds, 16 bytes a lane), into one of two images.  A block is multiplied in two
+// halves of 64: while the first multiplies out of registers, the second's fragments are read, after which the image is done with:
+// behind the block's one barrier, while the second half multiplies, the rows of the block after the next are asked for in its place and
+// the first fragments of the next block are read.  So a request has one and a half blocks of multiplication to arrive and a
+// read half a block; neither is waited for.  The 16-byte pieces of a row are stored in the order piece ^ (row & 7), so that eight
+// neighbouring rows' reads of one piece cover all banks.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ f32x16 mul32_fp8(i32x8 a, int sa, i32x8 b, int sb, f32x16 acc) {
@@ -270,36 +271,38 @@ __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane
 
 template <int ROWS>
 struct Stage {      // one operand's rows on their way into LDS
-    static constexpr int N = ROWS / 64;      // instructions of a wave per step, sixteen rows each
+    static constexpr int N = ROWS / 32;      // instructions of a wave per block, eight rows each
     const uint8_t* base;
     unsigned offset[N];      // of this lane's 16 bytes; rows behind the last stand for the last
     __device__ __forceinline__ Stage(const uint8_t* p, int64_t row0, int64_t rows, int64_t ldk) : base(p + row0 * ldk) {
         const int lane = threadIdx.x & 63, wave = wave_id();
         const int last = (int)(rows - row0 < ROWS ? rows - row0 : ROWS) - 1;
-        const int r = lane >> 2;
+        const int r = lane >> 3;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int row = 16 * (wave + 4 * i) + r;
-            offset[i] = (unsigned)(row < last ? row : last) * (unsigned)ldk + (((lane & 3) ^ (r >> 1 & 3)) << 4);
+            const int row = 8 * (wave + 4 * i) + r;
+            offset[i] = (unsigned)(row < last ? row : last) * (unsigned)ldk + (((lane & 7) ^ r) << 4);
         }
     }
-    __device__ __forceinline__ void issue(int i, int step, uint8_t* image) const {
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + (int64_t)step * KH + offset[i]),
-                                         (__attribute__((address_space(3))) void*)(image + 16 * (wave_id() + 4 * i) * KH), 16, 0, 0);
+    __device__ __forceinline__ void issue(int i, int kb, uint8_t* image) const {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + (int64_t)kb * KB + offset[i]),
+                                         (__attribute__((address_space(3))) void*)(image + 8 * (wave_id() + 4 * i) * KB), 16, 0, 0);
     }
 };
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-// where a lane's 32 of the 64 bytes of row `row` lie in an image: pieces 2 g and 2 g + 1
+// where a lane's 32 of the 64 bytes of either half of row `row` lie in an image: pieces 4 h + 2 g and the one behind it
 struct Piece {
-    int x, y;
+    int x[2], y[2];
     __device__ __forceinline__ Piece(int row, int g) {
-        const int sw = row >> 1 & 3;
-        x = row * KH + (((2 * g) ^ sw) << 4);
-        y = row * KH + (((2 * g + 1) ^ sw) << 4);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            x[h] = row * KB + (((4 * h + 2 * g) ^ (row & 7)) << 4);
+            y[h] = row * KB + (((4 * h + 2 * g + 1) ^ (row & 7)) << 4);
+        }
     }
-    __device__ __forceinline__ i32x8 read(const uint8_t* image, int t) const {      // of the row 32 t further (the order of its pieces is the same)
-        const i32x4 p = *reinterpret_cast<const i32x4*>(image + x + 32 * t * KH), q = *reinterpret_cast<const i32x4*>(image + y + 32 * t * KH);
+    __device__ __forceinline__ i32x8 read(const uint8_t* image, int h, int t) const {      // of the row 32 t further (the order of its pieces is the same)
+        const i32x4 p = *reinterpret_cast<const i32x4*>(image + x[h] + 32 * t * KB), q = *reinterpret_cast<const i32x4*>(image + y[h] + 32 * t * KB);
         return __builtin_shufflevector(p, q, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 };
@@ -375,8 +378,8 @@ __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, in
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[t][u][e] = 0.0f;
 
-    constexpr int IMAGE = (BM + BN) * KH, WORDS = (BM + BN) * 4;
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];      // four images, two sets of scale words
+    constexpr int IMAGE = (BM + BN) * KB, WORDS = (BM + BN) * 4;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];      // two images, two sets of scale words
     // the scales of four blocks are a word per row; a set of words comes along with the first image that needs it
     constexpr int SROWS = (BM + BN) / 4;      // rows of a wave
     const uint8_t* srow[SROWS / 64];
@@ -386,65 +389,48 @@ __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, in
         if (SROWS * wave + 64 * i < BM) srow[i] = p.sa + (i0 + row < p.m ? i0 + row : p.m - 1) * p.lds;
         else srow[i] = p.sb + (j0 + row - BM < p.n ? j0 + row - BM : p.n - 1) * p.lds;
     }
-    uint8_t* const words = lds + 4 * IMAGE;
+    uint8_t* const words = lds + 2 * IMAGE;
     auto issue_words = [&](int group) {
 #pragma unroll
         for (int i = 0; i < SROWS / 64; ++i)
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(srow[i] + 4 * (int64_t)group),
                                              (__attribute__((address_space(3))) void*)(words + (group & 1) * WORDS + (SROWS * wave + 64 * i) * 4), 4, 0, 0);
     };
-    const int s0 = 2 * kb0, s1 = 2 * kb1;
-    constexpr int NA = Stage<BM>::N, PER_STEP = NA + Stage<BN>::N;      // this wave's row instructions of a step
-    // (no branches: behind the last step its rows come once more, into an image that nobody reads any longer)
-    auto issue = [&](int i, int step) {
-        uint8_t* image = lds + (step & 3) * IMAGE;
-        const int from = step < s1 ? step : s1 - 1;
-        if (i < NA) sa.issue(i, from, image);
-        else sb.issue(i - NA, from, image + BM * KH);
+    constexpr int NA = Stage<BM>::N, N = NA + Stage<BN>::N;      // this wave's row instructions of a block
+    auto issue = [&](int i, int kb) {
+        uint8_t* image = lds + (kb & 1) * IMAGE;
+        if (i < NA) sa.issue(i, kb, image);
+        else sb.issue(i - NA, kb, image + BM * KB);
     };
     const Piece pa(wm + r, g), pb(wn + r, g);
-    i32x8 af[2][MT], bf[2][NT];
+    i32x8 a0[MT], b0[NT], a1[MT], b1[NT];
     unsigned wa[MT], wb[NT], na[MT], nb[NT];
-    auto fetch = [&](int i, int step, i32x8 (&a)[MT], i32x8 (&b)[NT]) {      // piece i of a step's MT + NT
-        const uint8_t* image = lds + (step & 3) * IMAGE;
-        if (i < MT) a[i] = pa.read(image, i);
-        else b[i - MT] = pb.read(image + BM * KH, i - MT);
+    auto fetch = [&](int i, int kb, int h, i32x8 (&a)[MT], i32x8 (&b)[NT]) {      // piece i of a half block's MT + NT
+        const uint8_t* image = lds + (kb & 1) * IMAGE;
+        if (i < MT) a[i] = pa.read(image, h, i);
+        else b[i - MT] = pb.read(image + BM * KB, h, i - MT);
     };
     auto fetch_words = [&](int kb) {
         const unsigned* w = reinterpret_cast<const unsigned*>(words + ((kb >> 2) & 1) * WORDS);
-        const int sh = 8 * (kb & 3);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) na[t] = w[wm + 32 * t + r] >> sh;
+        for (int t = 0; t < MT; ++t) na[t] = w[wm + 32 * t + r];
 #pragma unroll
-        for (int u = 0; u < NT; ++u) nb[u] = w[BM + wn + 32 * u + r] >> sh;
+        for (int u = 0; u < NT; ++u) nb[u] = w[BM + wn + 32 * u + r];
     };
-    // the rows of the step after this one are in LDS: those of the step behind it may still be out, and the scale words among them;
-    // and every wave is done with the image that is overwritten next
-    auto landed = [&] {
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER_STEP) : "memory");
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    // Step `step` multiplies out of a, b; between its instructions, in this order, the next step's fragments are read into an, bn and
-    // the rows of the step three ahead are asked for.  (One wave per SIMD: what is not placed between matrix instructions, which
-    // take 64 cycles each, is waited for.)
-    auto run = [&](int step, const i32x8 (&a)[MT], const i32x8 (&b)[NT], i32x8 (&an)[MT], i32x8 (&bn)[NT], auto also) {
-        constexpr int M = MT * NT, P = MT + NT;
+    // One half block multiplies out of a, b; between its instructions and in this order `beside(i)` places reads and requests.  (One wave
+    // per SIMD: what is not placed between matrix instructions, which take 64 cycles each, is waited for.)
+    auto multiply = [&](const i32x8 (&a)[MT], const i32x8 (&b)[NT], auto beside) {
+        constexpr int M = MT * NT;
         if constexpr (!F32) {
 #pragma unroll
             for (int i = 0; i < M; ++i) {
                 acc[i / NT][i % NT] = mul32_fp8(a[i / NT], (int)wa[i / NT], b[i % NT], (int)wb[i % NT], acc[i / NT][i % NT]);
-                if (i < P) fetch(i, step + 1, an, bn);
-                if (i >= M - PER_STEP) issue(i - (M - PER_STEP), step + 3);
-                if (i == (P < M ? P : M - 1)) also();
+                beside(i);
                 __builtin_amdgcn_sched_barrier(0);
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < P; ++i) fetch(i, step + 1, an, bn);
-#pragma unroll
-            for (int i = 0; i < PER_STEP; ++i) issue(i, step + 3);
-            also();
+            for (int i = 0; i < M; ++i) beside(i);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 bf16x8 ad[MT], bd[NT];
@@ -460,36 +446,53 @@ __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, in
             __builtin_amdgcn_sched_barrier(0);
         }
     };
+    auto block = [&](int kb, auto more) {      // more: there are two blocks behind this one
+        constexpr int M = MT * NT, P = MT + NT;      // P <= M: a piece beside each of the first P
+        static_assert(P <= M);
+        const int sh = 8 * (kb & 3);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) wa[t] = na[t] >> sh;
+#pragma unroll
+        for (int u = 0; u < NT; ++u) wb[u] = nb[u] >> sh;
+        multiply(a0, b0, [&](int i) {
+            if (i < P) fetch(i, kb, 1, a1, b1);
+        });
+        // this wave's rows of the next block are in LDS, then everyone's; and everyone is done with this one's image
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(a1, b1, [&](int i) {
+            if constexpr (decltype(more)::value) {
+                if (i == 0) issue_words((kb + 2) >> 2);
+#pragma unroll
+                for (int q = i * N / M; q < (i + 1) * N / M; ++q) issue(q, kb + 2);
+            }
+            if (i < P) fetch(i, kb + 1, 0, a0, b0);
+            if (i == M / 2) fetch_words(kb + 1);
+        });
+    };
     issue_words(kb0 >> 2);
 #pragma unroll
-    for (int i = 0; i < PER_STEP; ++i) issue(i, s0);
+    for (int i = 0; i < N; ++i) issue(i, kb0);
+    if (kb0 + 1 < kb1) {
+        issue_words((kb0 + 1) >> 2);
 #pragma unroll
-    for (int i = 0; i < PER_STEP; ++i) issue(i, s0 + 1);
-    issue_words((kb0 + 1 < kb1 ? kb0 + 1 : kb0) >> 2);
-#pragma unroll
-    for (int i = 0; i < PER_STEP; ++i) issue(i, s0 + 2);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER_STEP) : "memory");
+        for (int i = 0; i < N; ++i) issue(i, kb0 + 1);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+    } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
     asm volatile("s_barrier" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < MT + NT; ++i) fetch(i, s0, af[0], bf[0]);
+    for (int i = 0; i < MT + NT; ++i) fetch(i, kb0, 0, a0, b0);
     fetch_words(kb0);
-    for (int kb = kb0; kb < kb1; ++kb) {
-#pragma unroll
-        for (int t = 0; t < MT; ++t) wa[t] = na[t];
-#pragma unroll
-        for (int u = 0; u < NT; ++u) wb[u] = nb[u];
-        landed();
-        run(2 * kb, af[0], bf[0], af[1], bf[1], [] {});
-        landed();
-        issue_words((kb + 2 < kb1 ? kb + 2 : kb1 - 1) >> 2);
-        run(2 * kb + 1, af[1], bf[1], af[0], bf[0], [&] { fetch_words(kb + 1); });
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    int kb = kb0;
+    for (; kb + 2 < kb1; ++kb) block(kb, std::true_type{});
+    for (; kb < kb1; ++kb) block(kb, std::false_type{});      // (behind the last block an image's old rows are read and not used)
     // out through LDS, 32 rows of the wave's columns at a time, so that a store is 16 bytes of a row (or fp32 partial sums likewise)
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     asm volatile("s_barrier" ::: "memory");
     constexpr int COLS = 32 * NT, LD = COLS + 4;
-    static_assert(4 * 32 * LD * sizeof(float) <= 4 * IMAGE, "the bands of four waves lie in the images");
+    static_assert(4 * 32 * LD * sizeof(float) <= 2 * IMAGE, "the bands of four waves lie in the images");
     float* band_image = reinterpret_cast<float*>(lds) + wave * 32 * LD;
     const bool sums = partial != nullptr;
     const int64_t col0 = j0 + wn;
@@ -556,7 +559,7 @@ int product(const Product& p, int64_t k, int type, float* ws, hipStream_t stream
     if (plan.slices > 1 && !ws) return fail(NERF_E_ARG, "nerf_fp8_matmul: null workspace");
 #define GO(E)                                                                                                                        \
     do {                                                                                                                             \
-        constexpr size_t bytes = (E + E) * (4 * KH + 8);                                                                                 \
+        constexpr size_t bytes = (E + E) * (2 * KB + 8);                                                                                 \
         const hipError_t e = lds_limit_once((const void*)&k_product_tile<T, E, E>, bytes);                                           \
         if (e != hipSuccess) return fail(NERF_E_LAUNCH, "nerf_fp8_matmul: %s", hipGetErrorString(e));                                \
         hipLaunchKernelGGL((k_product_tile<T, E, E>), grid, dim3(256), bytes, stream, p, (int)tm, (int)tn, plan.blocks_per_slice, part); \

@@ -62,49 +62,69 @@ __device__ __forceinline__ unsigned pack4(float a, float b, float c, float d, fl
     return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(finite_or_nan(c) * inv, finite_or_nan(d) * inv, w, true);
 }
 
-constexpr int QT = 128;       // a workgroup quantises a tile of 128 x 128
-constexpr int QLD = QT + 1;
+constexpr int QT = 128;       // a workgroup quantises a tile of 128 x 128, a thread 8 x 8 of it
+constexpr int QLD = QT + 16;
+
+// the columns' largest (or sums) over the 16 threads that hold a column: 4 of a wave, then the waves through LDS
+template <typename Op>
+__device__ __forceinline__ void over_rows(unsigned (&v)[8], unsigned (*red)[QT], Op op) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        v[j] = op(v[j], (unsigned)__shfl_xor((int)v[j], 16));
+        v[j] = op(v[j], (unsigned)__shfl_xor((int)v[j], 32));
+    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = (lane & 15) * 8;
+    if (lane < 16) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) red[wave][c + j] = v[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = op(op(red[0][c + j], red[1][c + j]), op(red[2][c + j], red[3][c + j]));
+}
 
 // codes / scales: along the columns (rows keep their order); codes_t / scales_t: of the transpose, along the rows; colsum: sums of the
 // tile's columns, [tile row][cols].  mask: values whose mask entry is <= 0 count as 0 (the gradient of a ReLU's output).
+// One pass over x whatever is asked for; the transposed codes are packed along the rows in registers and cross the workgroup as bytes.
 template <typename T, bool ROWS, bool COLS>
 __global__ void __launch_bounds__(256) k_quantize(int64_t rows, int64_t cols, const T* __restrict__ x, int64_t ldx, int wide,
                                                   const T* __restrict__ mask, int64_t ldm, uint8_t* __restrict__ codes, int64_t ldc,
                                                   uint8_t* __restrict__ scales, int64_t lds, uint8_t* __restrict__ codes_t, int64_t ldct,
                                                   uint8_t* __restrict__ scales_t, int64_t ldst, float* __restrict__ colsum) {
-    extern __shared__ float tile[];       // [QT][QLD], only with COLS
-    const int64_t r0 = (int64_t)blockIdx.x * QT;
-    const int64_t c0 = (int64_t)blockIdx.y * QT;
-    const int tid = threadIdx.x, cl = (tid & 15) * 8;
+    const int64_t r0 = (int64_t)blockIdx.x * QT, c0 = (int64_t)blockIdx.y * QT;
+    const int tid = threadIdx.x, rl = (tid >> 4) * 8, cl = (tid & 15) * 8;
     const int64_t c = c0 + cl;
-#pragma unroll 2
+    float v[8][8];
+#pragma unroll
     for (int q = 0; q < 8; ++q) {
-        const int rl = (tid >> 4) + 16 * q;
-        const int64_t r = r0 + rl;
-        float v[8];
-        if (r < rows && wide && c + 8 <= cols) {
-            load_vec<T, 8>(x + r * ldx + c, v);
+        const int64_t r = r0 + rl + q;
+        if (wide && r < rows && c + 8 <= cols) {
+            load_vec<T, 8>(x + r * ldx + c, v[q]);
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = (r < rows && c + e < cols) ? (float)x[r * ldx + c + e] : 0.0f;
+            for (int e = 0; e < 8; ++e) v[q][e] = (r < rows && c + e < cols) ? (float)x[r * ldx + c + e] : 0.0f;
         }
-        if (mask) {
+    }
+    if (mask) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const int64_t r = r0 + rl + q;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (r < rows && c + e < cols && (float)mask[r * ldm + c + e] <= 0.0f) v[e] = 0.0f;
+                if (r < rows && c + e < cols && (float)mask[r * ldm + c + e] <= 0.0f) v[q][e] = 0.0f;
         }
-        if (COLS) {
+    }
+    if (ROWS) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) tile[rl * QLD + cl + e] = v[e];
-        }
-        if (ROWS) {
+        for (int q = 0; q < 8; ++q) {
+            const int64_t r = r0 + rl + q;
             unsigned am = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { const unsigned u = mag_bits(v[e]); am = u > am ? u : am; }
+            for (int e = 0; e < 8; ++e) { const unsigned u = mag_bits(v[q][e]); am = u > am ? u : am; }
             const int ex = scale_exp(row16_max(am));
             const float inv = pow2(-ex);
             if (r < rows) {
-                const uint2 w = make_uint2(pack4(v[0], v[1], v[2], v[3], inv), pack4(v[4], v[5], v[6], v[7], inv));
+                const uint2 w = make_uint2(pack4(v[q][0], v[q][1], v[q][2], v[q][3], inv), pack4(v[q][4], v[q][5], v[q][6], v[q][7], inv));
                 *reinterpret_cast<uint2*>(codes + r * ldc + c) = w;
                 if ((tid & 15) == 0) {
                     scales[r * lds + blockIdx.y] = (uint8_t)(ex + 127);
@@ -115,51 +135,72 @@ __global__ void __launch_bounds__(256) k_quantize(int64_t rows, int64_t cols, co
         }
     }
     if (!COLS) return;
-    __syncthreads();
-    const int col = tid >> 1, half = tid & 1;       // two neighbouring lanes share a column
-    const int64_t gc = c0 + col;
-    unsigned am = 0;
-    float sum = 0.0f;
-#pragma unroll 8
-    for (int k = 0; k < 64; ++k) {
-        const float v = tile[(64 * half + k) * QLD + col];
-        const unsigned u = mag_bits(v);
-        am = u > am ? u : am;
-        sum += v;
-    }
-    const unsigned am2 = (unsigned)__shfl_xor((int)am, 1);
-    sum += __shfl_xor(sum, 1);
-    am = am2 > am ? am2 : am;
-    if (gc >= cols) return;
-    if (colsum && half == 0) colsum[(int64_t)blockIdx.x * cols + gc] = sum;
-    if (!codes_t) return;
-    const int ex = scale_exp(am);
-    const float inv = pow2(-ex);
-    uint8_t* dst = codes_t + gc * ldct + r0 + 64 * half;
+    __shared__ unsigned red[2][4][QT];
+    if (colsum) {
+        unsigned sum[8];
 #pragma unroll
-    for (int k = 0; k < 64; k += 16) {
-        unsigned w[4];
+        for (int j = 0; j < 8; ++j) {
+            float t = v[0][j];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float* t = tile + (64 * half + k + 4 * j) * QLD + col;
-            w[j] = pack4(t[0], t[QLD], t[2 * QLD], t[3 * QLD], inv);
+            for (int q = 1; q < 8; ++q) t += v[q][j];
+            sum[j] = __float_as_uint(t);
         }
-        *reinterpret_cast<uint4*>(dst + k) = make_uint4(w[0], w[1], w[2], w[3]);
+        over_rows(sum, red[0], [](unsigned a, unsigned b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); });
+        if (tid < 16) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + j < cols) colsum[(int64_t)blockIdx.x * cols + c + j] = __uint_as_float(sum[j]);
+        }
     }
-    if (half == 0) {
-        scales_t[gc * ldst + blockIdx.x] = (uint8_t)(ex + 127);
-        if (blockIdx.x + 1 == gridDim.x)
-            for (int64_t z = blockIdx.x + 1; z < ldst; ++z) scales_t[gc * ldst + z] = 0;
+    if (!codes_t) return;
+    __shared__ __attribute__((aligned(16))) uint8_t bytes[QT * QLD];      // [column][row]
+    unsigned am[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        am[j] = 0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) { const unsigned u = mag_bits(v[q][j]); am[j] = u > am[j] ? u : am[j]; }
+    }
+    over_rows(am, red[1], [](unsigned a, unsigned b) { return a > b ? a : b; });
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int ex = scale_exp(am[j]);
+        const float inv = pow2(-ex);
+        const uint2 w = make_uint2(pack4(v[0][j], v[1][j], v[2][j], v[3][j], inv), pack4(v[4][j], v[5][j], v[6][j], v[7][j], inv));
+        *reinterpret_cast<uint2*>(bytes + (cl + j) * QLD + rl) = w;
+        if (tid < 16 && c + j < cols) {
+            scales_t[(c + j) * ldst + blockIdx.x] = (uint8_t)(ex + 127);
+            if (blockIdx.x + 1 == gridDim.x)
+                for (int64_t z = blockIdx.x + 1; z < ldst; ++z) scales_t[(c + j) * ldst + z] = 0;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int piece = tid + 256 * q, col = piece >> 3, k = (piece & 7) * 16;
+        if (c0 + col < cols) *reinterpret_cast<uint4*>(codes_t + (c0 + col) * ldct + r0 + k) = *reinterpret_cast<const uint4*>(bytes + col * QLD + k);
     }
 }
 
+// the tiles' sums of 64 columns, in fp64, sixteen tiles at a time
+constexpr int CF_ROWS = 16;
 template <typename T>
-__global__ void __launch_bounds__(256) k_colsum_finish(int64_t tiles, int64_t cols, const float* __restrict__ part, T* __restrict__ out) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= cols) return;
+__global__ void __launch_bounds__(64 * CF_ROWS) k_colsum_finish(int64_t tiles, int64_t cols, const float* __restrict__ part, T* __restrict__ out) {
+    __shared__ double red[CF_ROWS][64];
+    const int lane = threadIdx.x & 63, row = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
     double s = 0.0;
-    for (int64_t t = 0; t < tiles; ++t) s += (double)part[t * cols + c];
-    out[c] = (T)(float)s;
+    if (c < cols) {
+#pragma unroll 4
+        for (int64_t t = row; t < tiles; t += CF_ROWS) s += (double)part[t * cols + c];
+    }
+    red[row][lane] = s;
+    __syncthreads();
+    if (row == 0 && c < cols) {
+#pragma unroll
+        for (int k = 1; k < CF_ROWS; ++k) s += red[k][lane];
+        out[c] = (T)(float)s;
+    }
 }
 
 // ---- products -------------------------------------------------------------------------------------------------------------------
@@ -509,15 +550,43 @@ __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, in
     }
 }
 
-// c = act(sum over the slices of k, in their order, + bias)
+// c = act(sum over the slices of k + bias): four groups of 64 threads take a quarter of the slices each, in their order, and their sums
+// are added in theirs; a thread holds four values that follow one another in the partial sums
 template <typename T>
 __global__ void __launch_bounds__(256) k_product_join(Product p, int slices, const float* __restrict__ partial) {
-    const int64_t size = p.m * p.n;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
-        float s = 0.0f;
-        for (int z = 0; z < slices; ++z) s += partial[z * size + i];
-        const int64_t row = i / p.n, col = i - row * p.n;
-        ((T*)p.c)[row * p.ldc + col] = (T)finish<T>(s, p, col);
+    __shared__ float4 red[3][64];
+    const int lane = threadIdx.x & 63, group = threadIdx.x >> 6;
+    const int64_t size = p.m * p.n, i = ((int64_t)blockIdx.x * 64 + lane) * 4;
+    const int per = (slices + 3) / 4, z0 = group * per, z1 = z0 + per < slices ? z0 + per : slices;
+    float4 s = make_float4(0, 0, 0, 0);
+    if (i + 4 <= size && (size & 3) == 0) {
+#pragma unroll 8
+        for (int z = z0; z < z1; ++z) {
+            const float4 q = *reinterpret_cast<const float4*>(partial + z * size + i);
+            s.x += q.x; s.y += q.y; s.z += q.z; s.w += q.w;
+        }
+    } else {
+        float t[4] = {0, 0, 0, 0};
+        for (int z = z0; z < z1; ++z)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (i + e < size) t[e] += partial[z * size + i + e];
+        s = make_float4(t[0], t[1], t[2], t[3]);
+    }
+    if (group > 0) red[group - 1][lane] = s;
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+        const float4 o = red[q][lane];
+        s.x += o.x; s.y += o.y; s.z += o.z; s.w += o.w;
+    }
+    const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (i + e >= size) break;
+        const int64_t row = (i + e) / p.n, col = i + e - row * p.n;
+        ((T*)p.c)[row * p.ldc + col] = (T)finish<T>(v[e], p, col);
     }
 }
 
@@ -535,7 +604,7 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, int type) {
     const int tile = type != NERF_F32 && tiles(256) >= cus ? 256 : 128;
     int64_t slices = 1;
     const int64_t count = tiles(tile);
-    if (count < 2 * cus) slices = (2 * cus + count - 1) / count;
+    if (count < cus) slices = cus / count;
     if (slices > blocks / 4) slices = blocks / 4;
     if (slices < 1) slices = 1;
     const int64_t per = (blocks + slices - 1) / slices;
@@ -572,8 +641,7 @@ int product(const Product& p, int64_t k, int type, float* ws, hipStream_t stream
 #undef GO
     const int rc = launched("nerf_fp8_matmul");
     if (rc || !part) return rc;
-    const int64_t wgs = (p.m * p.n + 255) / 256;
-    hipLaunchKernelGGL((k_product_join<T>), dim3((unsigned)(wgs < 4096 ? wgs : 4096)), dim3(256), 0, stream, p, plan.slices, part);
+    hipLaunchKernelGGL((k_product_join<T>), dim3((unsigned)((p.m * p.n + 255) / 256)), dim3(256), 0, stream, p, plan.slices, part);
     return launched("nerf_fp8_matmul (join)");
 }
 
@@ -583,25 +651,18 @@ int quantize(int64_t rows, int64_t cols, const T* x, int64_t ldx, const T* mask,
     const int64_t ldc = code_stride(cols), lds = scale_stride(cols), ldct = code_stride(rows), ldst = scale_stride(rows);
     const dim3 grid((unsigned)((rows + QT - 1) / QT), (unsigned)((cols + QT - 1) / QT));
     const int wide = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(ldx * sizeof(T))) & 15) == 0;
-    const size_t bytes = sizeof(float) * QT * QLD;
     const bool cols_too = codes_t || col_sum;
 #define GO(R, C)                                                                                                                     \
-    do {                                                                                                                             \
-        if (C) {                                                                                                                     \
-            const hipError_t e = lds_limit_once((const void*)&k_quantize<T, R, C>, bytes);                                           \
-            if (e != hipSuccess) return fail(NERF_E_LAUNCH, "nerf_fp8_quantize: %s", hipGetErrorString(e));                          \
-        }                                                                                                                            \
-        hipLaunchKernelGGL((k_quantize<T, R, C>), grid, dim3(256), C ? bytes : 0, stream, rows, cols, x, ldx, wide, mask, ldm, codes, ldc, \
-                           scales, lds, codes_t, ldct, scales_t, ldst, col_sum ? ws : (float*)nullptr);                              \
-    } while (0)
+    hipLaunchKernelGGL((k_quantize<T, R, C>), grid, dim3(256), 0, stream, rows, cols, x, ldx, wide, mask, ldm, codes, ldc, scales, lds, \
+                       codes_t, ldct, scales_t, ldst, col_sum ? ws : (float*)nullptr)
     if (codes && cols_too) GO(true, true); else if (codes) GO(true, false); else GO(false, true);
 #undef GO
     const int rc = launched("nerf_fp8_quantize");
     if (rc || !col_sum) return rc;
-    const dim3 cgrid((unsigned)((cols + 255) / 256));
+    const dim3 cgrid((unsigned)((cols + 63) / 64));
     const int64_t tiles = (rows + QT - 1) / QT;
-    if (sum_type == NERF_F32) hipLaunchKernelGGL((k_colsum_finish<float>), cgrid, dim3(256), 0, stream, tiles, cols, ws, (float*)col_sum);
-    else hipLaunchKernelGGL((k_colsum_finish<T>), cgrid, dim3(256), 0, stream, tiles, cols, ws, (T*)col_sum);
+    if (sum_type == NERF_F32) hipLaunchKernelGGL((k_colsum_finish<float>), cgrid, dim3(64 * CF_ROWS), 0, stream, tiles, cols, ws, (float*)col_sum);
+    else hipLaunchKernelGGL((k_colsum_finish<T>), cgrid, dim3(64 * CF_ROWS), 0, stream, tiles, cols, ws, (T*)col_sum);
     return launched("nerf_fp8_quantize (sums)");
 }
 

@@ -83,35 +83,85 @@ __device__ __forceinline__ void over_rows(unsigned (&v)[8], unsigned (*red)[QT],
     for (int j = 0; j < 8; ++j) v[j] = op(op(red[0][c + j], red[1][c + j]), op(red[2][c + j], red[3][c + j]));
 }
 
+// Along the columns alone: sixteen lanes hold a block of 128, a workgroup 16 N blocks that follow one another in memory.
+template <typename T, int N>
+__global__ void __launch_bounds__(256) k_quantize_rows(int64_t rows, int64_t cols, const T* __restrict__ x, int64_t ldx, int wide,
+                                                       unsigned blocks, uint8_t* __restrict__ codes, int64_t ldc, uint8_t* __restrict__ scales,
+                                                       int64_t lds) {
+    const int l = threadIdx.x & 15;
+    const int64_t total = rows * blocks, first = (int64_t)blockIdx.x * (16 * N) + (threadIdx.x >> 4);
+    float v[N][8];
+    int64_t row[N];
+    unsigned kb[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+        const int64_t id = first + 16 * q;
+        row[q] = total <= 0xffffffffll ? (int64_t)((unsigned)id / blocks) : id / blocks;
+        kb[q] = (unsigned)(id - row[q] * blocks);
+        const int64_t c = (int64_t)kb[q] * KB + l * 8;
+        if (wide && row[q] < rows && c + 8 <= cols) {
+            load_vec<T, 8>(x + row[q] * ldx + c, v[q]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[q][e] = (row[q] < rows && c + e < cols) ? (float)x[row[q] * ldx + c + e] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+        unsigned am = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { const unsigned u = mag_bits(v[q][e]); am = u > am ? u : am; }
+        const int ex = scale_exp(row16_max(am));
+        const float inv = pow2(-ex);
+        if (row[q] >= rows) continue;
+        *reinterpret_cast<uint2*>(codes + row[q] * ldc + (int64_t)kb[q] * KB + l * 8) =
+            make_uint2(pack4(v[q][0], v[q][1], v[q][2], v[q][3], inv), pack4(v[q][4], v[q][5], v[q][6], v[q][7], inv));
+        if (l == 0) {
+            scales[row[q] * lds + kb[q]] = (uint8_t)(ex + 127);
+            if (kb[q] + 1 == blocks)
+                for (int64_t z = blocks; z < lds; ++z) scales[row[q] * lds + z] = 0;
+        }
+    }
+}
+
 // codes / scales: along the columns (rows keep their order); codes_t / scales_t: of the transpose, along the rows; colsum: sums of the
 // tile's columns, [tile row][cols].  mask: values whose mask entry is <= 0 count as 0 (the gradient of a ReLU's output).
 // One pass over x whatever is asked for; the transposed codes are packed along the rows in registers and cross the workgroup as bytes.
-template <typename T, bool ROWS, bool COLS>
-__global__ void __launch_bounds__(256) k_quantize(int64_t rows, int64_t cols, const T* __restrict__ x, int64_t ldx, int wide,
-                                                  const T* __restrict__ mask, int64_t ldm, uint8_t* __restrict__ codes, int64_t ldc,
+template <typename T, bool ROWS>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) k_quantize(int64_t rows, int64_t cols, unsigned col_tiles, const T* __restrict__ x, int64_t ldx, int wide,
+                                                  const T* __restrict__ mask, int64_t ldm, int wide_mask, uint8_t* __restrict__ codes, int64_t ldc,
                                                   uint8_t* __restrict__ scales, int64_t lds, uint8_t* __restrict__ codes_t, int64_t ldct,
                                                   uint8_t* __restrict__ scales_t, int64_t ldst, float* __restrict__ colsum) {
-    const int64_t r0 = (int64_t)blockIdx.x * QT, c0 = (int64_t)blockIdx.y * QT;
+    const unsigned row_tile = blockIdx.x / col_tiles, col_tile = blockIdx.x - row_tile * col_tiles, row_tiles = gridDim.x / col_tiles;
+    const int64_t r0 = (int64_t)row_tile * QT, c0 = (int64_t)col_tile * QT;
     const int tid = threadIdx.x, rl = (tid >> 4) * 8, cl = (tid & 15) * 8;
     const int64_t c = c0 + cl;
     float v[8][8];
+    const bool inside = wide && r0 + QT <= rows && c0 + QT <= cols;      // of the whole tile
+    const int nr = (int)(rows - r0 - rl < 8 ? rows - r0 - rl : 8), nc = (int)(cols - c < 8 ? cols - c : 8);      // this thread's valid part, possibly < 1
+    const T* src = x + (r0 + rl) * ldx + c;
+    if (inside) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-        const int64_t r = r0 + rl + q;
-        if (wide && r < rows && c + 8 <= cols) {
-            load_vec<T, 8>(x + r * ldx + c, v[q]);
-        } else {
+        for (int q = 0; q < 8; ++q) load_vec<T, 8>(src + q * ldx, v[q]);
+    } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[q][e] = (r < rows && c + e < cols) ? (float)x[r * ldx + c + e] : 0.0f;
-        }
+        for (int q = 0; q < 8; ++q)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[q][e] = (q < nr && e < nc) ? (float)src[q * ldx + e] : 0.0f;
     }
     if (mask) {
+        const T* gate = mask + (r0 + rl) * ldm + c;
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-            const int64_t r = r0 + rl + q;
+            float m[8];
+            if (inside && wide_mask) {
+                load_vec<T, 8>(gate + q * ldm, m);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (r < rows && c + e < cols && (float)mask[r * ldm + c + e] <= 0.0f) v[q][e] = 0.0f;
+                for (int e = 0; e < 8; ++e) m[e] = (q < nr && e < nc) ? (float)gate[q * ldm + e] : 1.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[q][e] = m[e] <= 0.0f ? 0.0f : v[q][e];
         }
     }
     if (ROWS) {
@@ -127,14 +177,13 @@ __global__ void __launch_bounds__(256) k_quantize(int64_t rows, int64_t cols, co
                 const uint2 w = make_uint2(pack4(v[q][0], v[q][1], v[q][2], v[q][3], inv), pack4(v[q][4], v[q][5], v[q][6], v[q][7], inv));
                 *reinterpret_cast<uint2*>(codes + r * ldc + c) = w;
                 if ((tid & 15) == 0) {
-                    scales[r * lds + blockIdx.y] = (uint8_t)(ex + 127);
-                    if (blockIdx.y + 1 == gridDim.y)
-                        for (int64_t z = blockIdx.y + 1; z < lds; ++z) scales[r * lds + z] = 0;
+                    scales[r * lds + col_tile] = (uint8_t)(ex + 127);
+                    if (col_tile + 1 == col_tiles)
+                        for (int64_t z = col_tiles; z < lds; ++z) scales[r * lds + z] = 0;
                 }
             }
         }
     }
-    if (!COLS) return;
     __shared__ unsigned red[2][4][QT];
     if (colsum) {
         unsigned sum[8];
@@ -149,7 +198,7 @@ __global__ void __launch_bounds__(256) k_quantize(int64_t rows, int64_t cols, co
         if (tid < 16) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (c + j < cols) colsum[(int64_t)blockIdx.x * cols + c + j] = __uint_as_float(sum[j]);
+                if (c + j < cols) colsum[(int64_t)row_tile * cols + c + j] = __uint_as_float(sum[j]);
         }
     }
     if (!codes_t) return;
@@ -169,9 +218,9 @@ __global__ void __launch_bounds__(256) k_quantize(int64_t rows, int64_t cols, co
         const uint2 w = make_uint2(pack4(v[0][j], v[1][j], v[2][j], v[3][j], inv), pack4(v[4][j], v[5][j], v[6][j], v[7][j], inv));
         *reinterpret_cast<uint2*>(bytes + (cl + j) * QLD + rl) = w;
         if (tid < 16 && c + j < cols) {
-            scales_t[(c + j) * ldst + blockIdx.x] = (uint8_t)(ex + 127);
-            if (blockIdx.x + 1 == gridDim.x)
-                for (int64_t z = blockIdx.x + 1; z < ldst; ++z) scales_t[(c + j) * ldst + z] = 0;
+            scales_t[(c + j) * ldst + row_tile] = (uint8_t)(ex + 127);
+            if (row_tile + 1 == row_tiles)
+                for (int64_t z = row_tiles; z < ldst; ++z) scales_t[(c + j) * ldst + z] = 0;
         }
     }
     __syncthreads();
@@ -649,14 +698,26 @@ template <typename T>
 int quantize(int64_t rows, int64_t cols, const T* x, int64_t ldx, const T* mask, int64_t ldm, uint8_t* codes, uint8_t* scales,
              uint8_t* codes_t, uint8_t* scales_t, int sum_type, void* col_sum, float* ws, hipStream_t stream) {
     const int64_t ldc = code_stride(cols), lds = scale_stride(cols), ldct = code_stride(rows), ldst = scale_stride(rows);
-    const dim3 grid((unsigned)((rows + QT - 1) / QT), (unsigned)((cols + QT - 1) / QT));
     const int wide = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(ldx * sizeof(T))) & 15) == 0;
-    const bool cols_too = codes_t || col_sum;
-#define GO(R, C)                                                                                                                     \
-    hipLaunchKernelGGL((k_quantize<T, R, C>), grid, dim3(256), 0, stream, rows, cols, x, ldx, wide, mask, ldm, codes, ldc, scales, lds, \
-                       codes_t, ldct, scales_t, ldst, col_sum ? ws : (float*)nullptr)
-    if (codes && cols_too) GO(true, true); else if (codes) GO(true, false); else GO(false, true);
+    const int wide_mask = ((reinterpret_cast<uintptr_t>(mask) | (uintptr_t)(ldm * sizeof(T))) & 15) == 0;
+    if (codes_t || col_sum || mask) {
+        const int64_t col_tiles = (cols + QT - 1) / QT, tiles_all = (rows + QT - 1) / QT * col_tiles;
+        if (tiles_all > 0xffffff) return fail(NERF_E_ARG, "nerf_fp8_quantize: %lld x %lld is more than one launch covers", (long long)rows, (long long)cols);
+#define GO(R)                                                                                                                        \
+    hipLaunchKernelGGL((k_quantize<T, R>), dim3((unsigned)tiles_all), dim3(256), 0, stream, rows, cols, (unsigned)col_tiles, x, ldx, wide, mask, \
+                       ldm, wide_mask, codes, ldc, scales, lds, codes_t, ldct, scales_t, ldst, col_sum ? ws : (float*)nullptr)
+        if (codes) GO(true); else GO(false);
 #undef GO
+    } else {
+        const int64_t blocks = blocks_of(cols), total = rows * blocks;
+        // four blocks a lane where that still fills the machine, one where latency counts
+        const int per = total >= 16 * 4 * 1024 ? 4 : 1;
+        const int64_t wgs = (total + 16 * per - 1) / (16 * per);
+        if (wgs > 0xffffff) return fail(NERF_E_ARG, "nerf_fp8_quantize: %lld x %lld is more than one launch covers", (long long)rows, (long long)cols);
+#define GO(N) hipLaunchKernelGGL((k_quantize_rows<T, N>), dim3((unsigned)wgs), dim3(256), 0, stream, rows, cols, x, ldx, wide, (unsigned)blocks, codes, ldc, scales, lds)
+        if (per == 4) GO(4); else GO(1);
+#undef GO
+    }
     const int rc = launched("nerf_fp8_quantize");
     if (rc || !col_sum) return rc;
     const dim3 cgrid((unsigned)((cols + 63) / 64));
@@ -680,7 +741,7 @@ int nerf_fp8_quantize(int64_t rows, int64_t cols, int type, const void* x, int64
     NERF_REQUIRE(rows >= 0 && cols >= 1, "nerf_fp8_quantize: rows=%lld cols=%lld", (long long)rows, (long long)cols);
     NERF_REQUIRE(elem_type_ok(type), "nerf_fp8_quantize: type=%d", type);
     NERF_REQUIRE(rows <= (int64_t)QT * 0x7fffff && cols <= (int64_t)QT * 65535, "nerf_fp8_quantize: %lld x %lld is more than one launch covers",
-                 (long long)rows, (long long)cols);
+                 (long long)rows, (long long)cols);      // (and the products of tiles below)
     NERF_REQUIRE(rows <= 1 || (ldx >= cols && (!mask || ldm >= cols)), "nerf_fp8_quantize: a row stride is less than cols=%lld", (long long)cols);
     if (rows == 0) return 0;
     NERF_REQUIRE(x && (!codes == !scales) && (!codes_t == !scales_t) && (codes || codes_t || col_sum) && (!col_sum || workspace),

@@ -13,8 +13,261 @@ using namespace nerfhip;
 namespace {
 
 constexpr int LN_THREADS = 256;
-constexpr int LN_SLICES = 256;      // slices of the rows in the weight gradients' sums
+constexpr int LN_SLICES = 1024;         // the most slices of the rows in the weight gradients' sums
+constexpr int64_t LN_HELD = 16384;      // rows up to this length are held in registers
 
+// a norm's weight or bias: fp32 or the rows' type, or absent
+template <typename T>
+struct Param {
+    const void* p;
+    int f32;
+    __device__ __forceinline__ float at(int64_t i, float absent) const {
+        return !p ? absent : f32 ? ((const float*)p)[i] : (float)((const T*)p)[i];
+    }
+};
+
+// VEC elements from any element's address (the memory system takes vector accesses at any alignment)
+template <typename T, int VEC>
+struct __attribute__((packed, aligned(sizeof(T)))) Loose { T e[VEC]; };
+template <typename T, int VEC>
+__device__ __forceinline__ Loose<T, VEC> read_raw(const T* row, int i, int c) {      // zeros behind c
+    if (i + VEC <= c) return *reinterpret_cast<const Loose<T, VEC>*>(row + i);
+    Loose<T, VEC> v;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v.e[e] = i + e < c ? row[i + e] : (T)0.0f;
+    return v;
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void read_row(const T* row, int i, int c, float (&out)[VEC]) {
+    const Loose<T, VEC> v = read_raw<T, VEC>(row, i, c);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) out[e] = (float)v.e[e];
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void write_row(T* row, int i, int c, const float (&in)[VEC]) {
+    if (i + VEC <= c) {
+        Loose<T, VEC> v;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v.e[e] = (T)in[e];
+        *reinterpret_cast<Loose<T, VEC>*>(row + i) = v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (i + e < c) row[i + e] = (T)in[e];
+    }
+}
+
+template <int CTRL>
+__device__ __forceinline__ float add_ror(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+
+// How a row is held: L lanes of WPR waves, VEC neighbouring elements at a time, CH times.
+template <int L_, int WPR_, int VEC_, int CH_>
+struct Shape {
+    static constexpr int L = L_, WPR = WPR_, VEC = VEC_, CH = CH_;
+    static constexpr int THREADS = WPR > 4 ? 64 * WPR : 256;
+    static constexpr int PER_ROW = L * WPR;                  // threads of a row
+    static constexpr int ROWS = THREADS / PER_ROW;           // rows a workgroup holds at once
+    static constexpr int MAX_C = PER_ROW * VEC * CH;
+    static constexpr int N = VEC * CH;
+};
+
+// the sum over a row's threads of K values, in every one of them; `part` holds K * WPR floats, another one for each call of an iteration
+template <typename S, int K>
+__device__ __forceinline__ void row_sum(float (&v)[K], float* part) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        if constexpr (S::L == 16) {
+            v[k] = add_ror<0x121>(v[k]);      // row_ror:1, 2, 4, 8
+            v[k] = add_ror<0x122>(v[k]);
+            v[k] = add_ror<0x124>(v[k]);
+            v[k] = add_ror<0x128>(v[k]);
+        } else {
+            v[k] = wave_sum_f32(v[k]);
+        }
+    }
+    if constexpr (S::WPR > 1) {
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) part[k * S::WPR + (threadIdx.x >> 6)] = v[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float t = part[k * S::WPR];
+#pragma unroll
+            for (int w = 1; w < S::WPR; ++w) t += part[k * S::WPR + w];
+            v[k] = t;
+        }
+    }
+}
+
+// One pass over memory: a row is read once, held in registers for both passes of the statistics, and written once.
+template <typename T, typename S>
+__global__ void __launch_bounds__(S::THREADS) k_ln_fwd_held(int64_t n, int c, const T* __restrict__ x, int64_t ldx, Param<T> w, Param<T> b, float eps,
+                                                            T* __restrict__ y, int64_t ldy, float* __restrict__ stats) {
+    __shared__ float part[2][2 * S::WPR];
+    const int lane = threadIdx.x % S::PER_ROW, slot = threadIdx.x / S::PER_ROW;
+    const float fc = (float)c;
+    for (int64_t row0 = (int64_t)blockIdx.x * S::ROWS; row0 < n; row0 += (int64_t)gridDim.x * S::ROWS) {
+        const int64_t row = row0 + slot;
+        const bool live = row < n;
+        const T* xr = x + (live ? row : n - 1) * ldx;
+        float v[S::CH][S::VEC], s[1] = {0.0f};
+#pragma unroll
+        for (int k = 0; k < S::CH; ++k) read_row<T, S::VEC>(xr, (k * S::PER_ROW + lane) * S::VEC, c, v[k]);
+#pragma unroll
+        for (int k = 0; k < S::CH; ++k)
+#pragma unroll
+            for (int e = 0; e < S::VEC; ++e) s[0] += v[k][e];
+        row_sum<S, 1>(s, part[0]);
+        const float mu1 = s[0] / fc;
+        float d[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < S::CH; ++k) {
+            const int i = (k * S::PER_ROW + lane) * S::VEC;
+#pragma unroll
+            for (int e = 0; e < S::VEC; ++e) {
+                v[k][e] = i + e < c ? v[k][e] - mu1 : 0.0f;
+                d[0] += v[k][e];
+                d[1] += v[k][e] * v[k][e];
+            }
+        }
+        row_sum<S, 2>(d, part[1]);
+        const float mu2 = d[0] / fc, var = fmaxf(d[1] / fc - mu2 * mu2, 0.0f);
+        const float r = (d[1] != d[1]) ? d[1] : 1.0f / sqrtf(var + eps);      // (fmaxf drops a NaN)
+        if (live) {
+#pragma unroll
+            for (int k = 0; k < S::CH; ++k) {
+                const int i = (k * S::PER_ROW + lane) * S::VEC;
+                if (i >= c) continue;
+                float o[S::VEC], wv[S::VEC], bv[S::VEC];
+#pragma unroll
+                for (int e = 0; e < S::VEC; ++e) { wv[e] = 1.0f; bv[e] = 0.0f; }
+                if (w.p) { if (w.f32) read_row<float, S::VEC>((const float*)w.p, i, c, wv); else read_row<T, S::VEC>((const T*)w.p, i, c, wv); }
+                if (b.p) { if (b.f32) read_row<float, S::VEC>((const float*)b.p, i, c, bv); else read_row<T, S::VEC>((const T*)b.p, i, c, bv); }
+#pragma unroll
+                for (int e = 0; e < S::VEC; ++e) o[e] = (v[k][e] - mu2) * r * wv[e] + bv[e];
+                write_row<T, S::VEC>(y + row * ldy, i, c, o);
+            }
+            if (stats && lane == 0) {
+                stats[row] = mu1;
+                stats[n + row] = mu2;
+                stats[2 * n + row] = r;
+            }
+        }
+    }
+}
+
+// x and dy are read once: dx is written and the weight's and bias's sums of this workgroup's rows stay in registers; they are left as
+// partial[workgroup][0 | 1][column].
+template <typename T, typename S>
+__global__ void __launch_bounds__(S::THREADS) k_ln_bwd_held(int64_t n, int c, const T* __restrict__ x, int64_t ldx, const T* __restrict__ dy,
+                                                            int64_t lddy, Param<T> w, const float* __restrict__ stats, T* __restrict__ dx,
+                                                            int64_t lddx, float* __restrict__ partial) {
+    __shared__ float part[2][2 * S::WPR];
+    const int lane = threadIdx.x % S::PER_ROW, slot = threadIdx.x / S::PER_ROW;
+    const float fc = (float)c;
+    float wv[S::CH][S::VEC], sw[S::CH][S::VEC], sb[S::CH][S::VEC];
+#pragma unroll
+    for (int k = 0; k < S::CH; ++k) {
+        const int i = (k * S::PER_ROW + lane) * S::VEC;
+#pragma unroll
+        for (int e = 0; e < S::VEC; ++e) {
+            wv[k][e] = i + e < c ? w.at(i + e, 1.0f) : 0.0f;
+            sw[k][e] = sb[k][e] = 0.0f;
+        }
+    }
+    // (the next row is under way while this one is worked on)
+    Loose<T, S::VEC> nx[S::CH], ng[S::CH];
+    auto request = [&](int64_t row) {
+        const int64_t at = row < n ? row : n - 1;
+#pragma unroll
+        for (int k = 0; k < S::CH; ++k) {
+            const int i = (k * S::PER_ROW + lane) * S::VEC;
+            nx[k] = read_raw<T, S::VEC>(x + at * ldx, i, c);
+            ng[k] = read_raw<T, S::VEC>(dy + at * lddy, i, c);
+        }
+    };
+    request((int64_t)blockIdx.x * S::ROWS + slot);
+    int odd = 0;
+    for (int64_t row0 = (int64_t)blockIdx.x * S::ROWS; row0 < n; row0 += (int64_t)gridDim.x * S::ROWS, odd ^= 1) {
+        const int64_t row = row0 + slot;
+        const bool live = row < n;
+        const int64_t at = live ? row : n - 1;
+        const float mu1 = stats[at], mu2 = stats[n + at], r = stats[2 * n + at];
+        float xh[S::CH][S::VEC], g[S::CH][S::VEC], s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < S::CH; ++k)
+#pragma unroll
+            for (int e = 0; e < S::VEC; ++e) {
+                xh[k][e] = (float)nx[k].e[e];
+                g[k][e] = (float)ng[k].e[e];
+            }
+        if (row0 + (int64_t)gridDim.x * S::ROWS < n) request(row + (int64_t)gridDim.x * S::ROWS);
+#pragma unroll
+        for (int k = 0; k < S::CH; ++k) {
+            const int i = (k * S::PER_ROW + lane) * S::VEC;
+#pragma unroll
+            for (int e = 0; e < S::VEC; ++e) {
+                xh[k][e] = i + e < c ? (xh[k][e] - mu1 - mu2) * r : 0.0f;
+                if (live) {
+                    sw[k][e] += g[k][e] * xh[k][e];
+                    sb[k][e] += g[k][e];
+                }
+                g[k][e] *= wv[k][e];
+                s[0] += g[k][e];
+                s[1] += g[k][e] * xh[k][e];
+            }
+        }
+        if (!dx) continue;
+        row_sum<S, 2>(s, part[odd]);
+        const float ma = s[0] / fc, mq = s[1] / fc;
+        if (live) {
+#pragma unroll
+            for (int k = 0; k < S::CH; ++k) {
+                const int i = (k * S::PER_ROW + lane) * S::VEC;
+                if (i >= c) continue;
+                float o[S::VEC];
+#pragma unroll
+                for (int e = 0; e < S::VEC; ++e) o[e] = r * (g[k][e] - ma - xh[k][e] * mq);
+                write_row<T, S::VEC>(dx + row * lddx, i, c, o);
+            }
+        }
+    }
+    if (!partial) return;
+    // the workgroup's rows' sums together, in their order
+    float* out = partial + (int64_t)blockIdx.x * 2 * c;
+    if constexpr (S::ROWS > 1) {
+        __shared__ float all[S::ROWS][S::MAX_C];
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < S::CH; ++k)
+#pragma unroll
+                for (int e = 0; e < S::VEC; ++e) all[slot][(k * S::PER_ROW + lane) * S::VEC + e] = which ? sb[k][e] : sw[k][e];
+            __syncthreads();
+            for (int i = threadIdx.x; i < c; i += S::THREADS) {
+                float t = all[0][i];
+#pragma unroll
+                for (int q = 1; q < S::ROWS; ++q) t += all[q][i];
+                out[(int64_t)which * c + i] = t;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < S::CH; ++k) {
+            const int i = (k * S::PER_ROW + lane) * S::VEC;
+            if (i >= c) continue;
+            write_row<float, S::VEC>(out, i, c, sw[k]);
+            write_row<float, S::VEC>(out + c, i, c, sb[k]);
+        }
+    }
+}
+
+// ---- rows too long for registers: read again for every pass
 __device__ __forceinline__ float block_sum(float v, float* part) {
     v = wave_sum_f32(v);
     __syncthreads();
@@ -26,9 +279,9 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
     return t;
 }
 
-template <typename T, typename W>
-__global__ void __launch_bounds__(LN_THREADS) k_ln_fwd(int64_t n, int c, const T* __restrict__ x, int64_t ldx, const W* __restrict__ w,
-                                                       const W* __restrict__ b, float eps, T* __restrict__ y, int64_t ldy,
+template <typename T>
+__global__ void __launch_bounds__(LN_THREADS) k_ln_fwd(int64_t n, int c, const T* __restrict__ x, int64_t ldx, Param<T> w,
+                                                       Param<T> b, float eps, T* __restrict__ y, int64_t ldy,
                                                        float* __restrict__ stats) {
     __shared__ float part[LN_THREADS / 64];
     for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
@@ -43,12 +296,12 @@ __global__ void __launch_bounds__(LN_THREADS) k_ln_fwd(int64_t n, int c, const T
             d2 += d * d;
         }
         const float mu2 = block_sum(d1, part) / (float)c;
-        const float var = fmaxf(block_sum(d2, part) / (float)c - mu2 * mu2, 0.0f);
-        const float r = 1.0f / sqrtf(var + eps);
+        d2 = block_sum(d2, part);
+        const float var = fmaxf(d2 / (float)c - mu2 * mu2, 0.0f);
+        const float r = (d2 != d2) ? d2 : 1.0f / sqrtf(var + eps);      // (fmaxf drops a NaN)
         for (int i = threadIdx.x; i < c; i += LN_THREADS) {
             float v = ((float)xr[i] - mu1 - mu2) * r;
-            if (w) v *= (float)w[i];
-            if (b) v += (float)b[i];
+            v = v * w.at(i, 1.0f) + b.at(i, 0.0f);
             y[row * ldy + i] = (T)v;
         }
         if (stats && threadIdx.x == 0) {
@@ -59,9 +312,9 @@ __global__ void __launch_bounds__(LN_THREADS) k_ln_fwd(int64_t n, int c, const T
     }
 }
 
-template <typename T, typename W>
+template <typename T>
 __global__ void __launch_bounds__(LN_THREADS) k_ln_dx(int64_t n, int c, const T* __restrict__ x, int64_t ldx, const T* __restrict__ dy,
-                                                      int64_t lddy, const W* __restrict__ w, const float* __restrict__ stats,
+                                                      int64_t lddy, Param<T> w, const float* __restrict__ stats,
                                                       T* __restrict__ dx, int64_t lddx) {
     __shared__ float part[LN_THREADS / 64];
     for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
@@ -69,13 +322,13 @@ __global__ void __launch_bounds__(LN_THREADS) k_ln_dx(int64_t n, int c, const T*
         const T *xr = x + row * ldx, *gr = dy + row * lddy;
         float a = 0.0f, q = 0.0f;
         for (int i = threadIdx.x; i < c; i += LN_THREADS) {
-            const float g = (float)gr[i] * (w ? (float)w[i] : 1.0f);
+            const float g = (float)gr[i] * w.at(i, 1.0f);
             a += g;
             q += g * (((float)xr[i] - mu1 - mu2) * r);
         }
         const float ma = block_sum(a, part) / (float)c, mq = block_sum(q, part) / (float)c;
         for (int i = threadIdx.x; i < c; i += LN_THREADS) {
-            const float g = (float)gr[i] * (w ? (float)w[i] : 1.0f);
+            const float g = (float)gr[i] * w.at(i, 1.0f);
             dx[row * lddx + i] = (T)(r * (g - ma - (((float)xr[i] - mu1 - mu2) * r) * mq));
         }
     }
@@ -99,49 +352,106 @@ __global__ void __launch_bounds__(LN_THREADS) k_ln_dw(int64_t n, int c, const T*
     partial[((int64_t)blockIdx.y * 2 + 1) * c + col] = sb;
 }
 
+// the slices' sums of 64 columns (of dw's C, then db's), in fp64, sixteen slices at a time
+constexpr int LF_ROWS = 16;
 template <typename W>
-__global__ void __launch_bounds__(LN_THREADS) k_ln_finish(int slices, int c, const float* __restrict__ partial, W* __restrict__ dw,
-                                                          W* __restrict__ db) {
-    const int col = blockIdx.x * LN_THREADS + threadIdx.x;
-    if (col >= c) return;
-    double sw = 0.0, sb = 0.0;
-    for (int z = 0; z < slices; ++z) {
-        sw += (double)partial[((int64_t)z * 2) * c + col];
-        sb += (double)partial[((int64_t)z * 2 + 1) * c + col];
+__global__ void __launch_bounds__(64 * LF_ROWS) k_ln_finish(int slices, int c, const float* __restrict__ partial, W* __restrict__ dw,
+                                                            W* __restrict__ db) {
+    __shared__ double red[LF_ROWS][64];
+    const int lane = threadIdx.x & 63, row = threadIdx.x >> 6;
+    const int64_t col = (int64_t)blockIdx.x * 64 + lane;
+    double s = 0.0;
+    if (col < 2 * (int64_t)c) {
+#pragma unroll 4
+        for (int z = row; z < slices; z += LF_ROWS) s += (double)partial[(int64_t)z * 2 * c + col];
     }
-    if (dw) dw[col] = (W)(float)sw;
-    if (db) db[col] = (W)(float)sb;
+    red[row][lane] = s;
+    __syncthreads();
+    if (row > 0 || col >= 2 * (int64_t)c) return;
+#pragma unroll
+    for (int k = 1; k < LF_ROWS; ++k) s += red[k][lane];
+    if (col < c) {
+        if (dw) dw[col] = (W)(float)s;
+    } else if (db) {
+        db[col - c] = (W)(float)s;
+    }
 }
 
-int slices_of(int64_t n) { return (int)(n < LN_SLICES ? (n < 1 ? 1 : n) : LN_SLICES); }
+// The shape that holds rows of c elements: the fewest lanes at first (short rows: several to a wave), then more elements a lane, then
+// more waves: 16 elements a lane of x, dy, the weight, both sums and the next row are what leaves four waves to a SIMD.
+template <typename F>
+int with_shape(int64_t c, F&& f) {
+    if (c <= 64) return f(Shape<16, 1, 4, 1>{});
+    if (c <= 128) return f(Shape<64, 1, 2, 1>{});
+    if (c <= 256) return f(Shape<64, 1, 4, 1>{});
+    if (c <= 512) return f(Shape<64, 1, 8, 1>{});
+    if (c <= 1024) return f(Shape<64, 1, 8, 2>{});
+    if (c <= 2048) return f(Shape<64, 4, 8, 1>{});
+    if (c <= 4096) return f(Shape<64, 4, 8, 2>{});
+    if (c <= 8192) return f(Shape<64, 8, 8, 2>{});
+    return f(Shape<64, 16, 8, 2>{});
+}
 
-template <typename T, typename W>
-int fwd(int64_t n, int c, const void* x, int64_t ldx, const void* w, const void* b, float eps, void* y, int64_t ldy, float* stats,
+// workgroups of the backward pass, each of which leaves one slice of the weight's gradient: enough to fill the machine, few enough
+// that the slices (8 bytes a column each) stay a small part of the rows' own traffic
+int slices_of(int64_t n, int64_t c) {
+    if (n < 1) return 1;
+    const int rows = c > LN_HELD ? 1 : with_shape(c, [](auto s) { return decltype(s)::ROWS; });
+    const int64_t groups = (n + rows - 1) / rows, most = c <= 2048 ? LN_SLICES : LN_SLICES / 2;
+    return (int)(groups < most ? groups : most);
+}
+
+template <typename T>
+int fwd(int64_t n, int c, const void* x, int64_t ldx, int w_f32, const void* w, const void* b, float eps, void* y, int64_t ldy, float* stats,
         hipStream_t stream) {
-    const unsigned grid = (unsigned)(n < 65536 ? n : 65536);
-    hipLaunchKernelGGL((k_ln_fwd<T, W>), dim3(grid), dim3(LN_THREADS), 0, stream, n, c, (const T*)x, ldx, (const W*)w, (const W*)b, eps,
-                       (T*)y, ldy, stats);
-    return launched("nerf_layer_norm_fwd");
+    const Param<T> wp{w, w_f32}, bp{b, w_f32};
+    if (c > LN_HELD) {
+        hipLaunchKernelGGL((k_ln_fwd<T>), dim3((unsigned)(n < 65536 ? n : 65536)), dim3(LN_THREADS), 0, stream, n, c, (const T*)x, ldx, wp, bp, eps,
+                           (T*)y, ldy, stats);
+        return launched("nerf_layer_norm_fwd");
+    }
+    return with_shape(c, [&](auto shape) {
+        using S = decltype(shape);
+        const int64_t groups = (n + S::ROWS - 1) / S::ROWS;
+        hipLaunchKernelGGL((k_ln_fwd_held<T, S>), dim3((unsigned)(groups < 8192 ? groups : 8192)), dim3(S::THREADS), 0, stream, n, c, (const T*)x,
+                           ldx, wp, bp, eps, (T*)y, ldy, stats);
+        return launched("nerf_layer_norm_fwd");
+    });
 }
 
-template <typename T, typename W>
-int bwd(int64_t n, int c, const void* x, int64_t ldx, const void* dy, int64_t lddy, const void* w, const float* stats, void* dx,
+template <typename T>
+int bwd(int64_t n, int c, const void* x, int64_t ldx, const void* dy, int64_t lddy, int w_f32, const void* w, const float* stats, void* dx,
         int64_t lddx, void* dw, void* db, float* ws, hipStream_t stream) {
-    if (dx && n > 0) {
-        const unsigned grid = (unsigned)(n < 65536 ? n : 65536);
-        hipLaunchKernelGGL((k_ln_dx<T, W>), dim3(grid), dim3(LN_THREADS), 0, stream, n, c, (const T*)x, ldx, (const T*)dy, lddy,
-                           (const W*)w, stats, (T*)dx, lddx);
-        const int rc = launched("nerf_layer_norm_bwd");
-        if (rc) return rc;
+    const Param<T> wp{w, w_f32};
+    const int slices = slices_of(n, c);
+    float* part = dw || db ? ws : nullptr;
+    if (!dx && !part) return 0;
+    int rc = 0;
+    if (c > LN_HELD || n == 0) {
+        const unsigned cols = (unsigned)((c + LN_THREADS - 1) / LN_THREADS);
+        if (dx && n > 0) {
+            hipLaunchKernelGGL((k_ln_dx<T>), dim3((unsigned)(n < 65536 ? n : 65536)), dim3(LN_THREADS), 0, stream, n, c, (const T*)x, ldx,
+                               (const T*)dy, lddy, wp, stats, (T*)dx, lddx);
+            rc = launched("nerf_layer_norm_bwd");
+            if (rc) return rc;
+        }
+        if (part) {
+            hipLaunchKernelGGL((k_ln_dw<T>), dim3(cols, slices), dim3(LN_THREADS), 0, stream, n, c, (const T*)x, ldx, (const T*)dy, lddy, stats,
+                               (n + slices - 1) / slices, part);
+            rc = launched("nerf_layer_norm_bwd (partial sums)");
+        }
+    } else {
+        rc = with_shape(c, [&](auto shape) {
+            using S = decltype(shape);
+            hipLaunchKernelGGL((k_ln_bwd_held<T, S>), dim3((unsigned)slices), dim3(S::THREADS), 0, stream, n, c, (const T*)x, ldx, (const T*)dy,
+                               lddy, wp, stats, (T*)dx, lddx, part);
+            return launched("nerf_layer_norm_bwd");
+        });
     }
-    if (!dw && !db) return 0;
-    const int slices = slices_of(n);
-    const unsigned cols = (unsigned)((c + LN_THREADS - 1) / LN_THREADS);
-    hipLaunchKernelGGL((k_ln_dw<T>), dim3(cols, slices), dim3(LN_THREADS), 0, stream, n, c, (const T*)x, ldx, (const T*)dy, lddy, stats,
-                       (n + slices - 1) / slices, ws);
-    const int rc = launched("nerf_layer_norm_bwd (partial sums)");
-    if (rc) return rc;
-    hipLaunchKernelGGL((k_ln_finish<W>), dim3(cols), dim3(LN_THREADS), 0, stream, slices, c, ws, (W*)dw, (W*)db);
+    if (rc || !part) return rc;
+    const dim3 grid((unsigned)((2 * (int64_t)c + 63) / 64));
+    if (w_f32) hipLaunchKernelGGL((k_ln_finish<float>), grid, dim3(64 * LF_ROWS), 0, stream, slices, c, part, (float*)dw, (float*)db);
+    else hipLaunchKernelGGL((k_ln_finish<T>), grid, dim3(64 * LF_ROWS), 0, stream, slices, c, part, (T*)dw, (T*)db);
     return launched("nerf_layer_norm_bwd (sums)");
 }
 
@@ -159,15 +469,14 @@ int nerf_layer_norm_fwd(int64_t n, int64_t c, int type, const void* x, int64_t l
     if (n == 0) return 0;
     NERF_REQUIRE(x && y, "nerf_layer_norm_fwd: null pointer");
     hipStream_t stream = as_stream(stream_);
-#define GO(T, W) return fwd<T, W>(n, (int)c, x, ldx, w, b, (float)eps, y, ldy, stats, stream)
-    if (type == NERF_F32) GO(float, float);
-    if (type == NERF_BF16) { if (w_type == NERF_F32) GO(bf16_t, float); GO(bf16_t, bf16_t); }
-    if (w_type == NERF_F32) GO(f16_t, float);
-    GO(f16_t, f16_t);
+#define GO(T) return fwd<T>(n, (int)c, x, ldx, w_type == NERF_F32, w, b, (float)eps, y, ldy, stats, stream)
+    if (type == NERF_F32) GO(float);
+    if (type == NERF_BF16) GO(bf16_t);
+    GO(f16_t);
 #undef GO
 }
 
-int64_t nerf_layer_norm_workspace_floats(int64_t n, int64_t c) { return (int64_t)slices_of(n) * 2 * (c < 0 ? 0 : c); }
+int64_t nerf_layer_norm_workspace_floats(int64_t n, int64_t c) { return c < 1 ? 0 : (int64_t)slices_of(n, c) * 2 * c; }
 
 int nerf_layer_norm_bwd(int64_t n, int64_t c, int type, const void* x, int64_t ldx, const void* dy, int64_t lddy, int w_type,
                         const void* w, const float* stats, void* dx, int64_t lddx, void* dw, void* db, float* workspace, void* stream_) {
@@ -177,11 +486,10 @@ int nerf_layer_norm_bwd(int64_t n, int64_t c, int type, const void* x, int64_t l
     NERF_REQUIRE(n == 0 || (x && dy && stats), "nerf_layer_norm_bwd: null pointer");
     NERF_REQUIRE(!(dw || db) || workspace, "nerf_layer_norm_bwd: null workspace");
     hipStream_t stream = as_stream(stream_);
-#define GO(T, W) return bwd<T, W>(n, (int)c, x, ldx, dy, lddy, w, stats, dx, lddx, dw, db, workspace, stream)
-    if (type == NERF_F32) GO(float, float);
-    if (type == NERF_BF16) { if (w_type == NERF_F32) GO(bf16_t, float); GO(bf16_t, bf16_t); }
-    if (w_type == NERF_F32) GO(f16_t, float);
-    GO(f16_t, f16_t);
+#define GO(T) return bwd<T>(n, (int)c, x, ldx, dy, lddy, w_type == NERF_F32, w, stats, dx, lddx, dw, db, workspace, stream)
+    if (type == NERF_F32) GO(float);
+    if (type == NERF_BF16) GO(bf16_t);
+    GO(f16_t);
 #undef GO
 }
 

@@ -407,7 +407,8 @@ int nerf_layer_norm_bwd(int64_t n, int64_t c, int type, const void* x, int64_t l
  *   scales_t of its transpose (both or neither NULL), every value rounded to nearest even once, e the smallest exponent (>= -126)
  *   with max |x| <= 448 * 2^e over the block; a value that is not finite becomes NaN and has no part in its block's scale.  mask
  *   (or NULL; of `type`, row stride ldm): x counts as 0 where mask <= 0.  col_sum (or NULL): [cols] of sum_type, the sums of the
- *   columns of the (masked) x; it takes a workspace of nerf_fp8_quantize_workspace_floats(rows, cols) floats.
+ *   columns of the (masked) x; it takes a workspace of nerf_fp8_quantize_workspace_floats(rows, cols) floats.  (mask without col_sum
+ *   is allowed; rows and columns behind the last are not read.)
  * nerf_fp8_matmul: c [m, n] of `type`, row stride ldc, = act(a [m, k] b [n, k]^T + bias [n]); bias (of bias_type: `type` or
  *   NERF_F32) may be NULL; relu != 0 applies max(., 0) (a NaN stays).  Sums in fp32: for an fp32 c by the bf16 matrix instruction
  *   on decoded values (products exact), for a 16-bit c by the scaled fp8 instruction, which cuts the products of eight consecutive
@@ -423,6 +424,24 @@ int64_t nerf_fp8_matmul_workspace_floats(int64_t m, int64_t n, int64_t k, int ty
 int nerf_fp8_matmul(int64_t m, int64_t n, int64_t k, const uint8_t* a, const uint8_t* a_scales, const uint8_t* b,
                     const uint8_t* b_scales, int bias_type, const void* bias, int relu, int type, void* c, int64_t ldc,
                     float* workspace, void* stream);
+
+/* A whole linear layer on such products (ops.linear_fp8): y [n, n_out] = act(x w^T + bias) and its gradients, one call each, every
+ * operand quantised along the k of its product: y = q(x) q(w)^T, dx = q(dy) q(w^T)^T, dw = q(dy^T) q(x^T)^T, db = column sums of dy
+ * (dy counts as 0 where y <= 0, if y is given: the gradient of the ReLU).  x, y, dy, dx of `type`; w [n_out, n_in] of w_type with
+ * row stride ldw, or, with w = NULL, held in 8 bits as w_codes / w_scales; bias, db of bias_type; each of w_type and bias_type
+ * `type` or NERF_F32.  y, dx, dw are dense.
+ * kept: what the backward pass needs, left by the forward (NULL: none; needs_dx / needs_dw say for which gradients),
+ *   nerf_linear_fp8_kept_bytes(n, n_in, n_out, needs_dx, needs_dw) bytes.  In the backward pass dx, dw, db may each be NULL;
+ *   needs_dx / needs_dw are those of the forward.  workspace: nerf_linear_fp8_workspace_bytes(n, n_in, n_out, type, w_type, backward) bytes,
+ *   contents irrelevant.  kept and workspace start at a multiple of 256 bytes. */
+int64_t nerf_linear_fp8_kept_bytes(int64_t n, int64_t n_in, int64_t n_out, int needs_dx, int needs_dw);
+int64_t nerf_linear_fp8_workspace_bytes(int64_t n, int64_t n_in, int64_t n_out, int type, int w_type, int backward);
+int nerf_linear_fp8_fwd(int64_t n, int64_t n_in, int64_t n_out, int type, const void* x, int64_t ldx, int w_type, const void* w,
+                        int64_t ldw, const uint8_t* w_codes, const uint8_t* w_scales, int bias_type, const void* bias, int relu,
+                        void* y, void* kept, int needs_dx, int needs_dw, void* workspace, void* stream);
+int nerf_linear_fp8_bwd(int64_t n, int64_t n_in, int64_t n_out, int type, const void* dy, int64_t lddy, const void* y,
+                        const void* kept, int needs_dx, int needs_dw, void* dx, int w_type, void* dw, int bias_type, void* db,
+                        void* workspace, void* stream);
 
 /* AdamW (decoupled weight decay) over n_tensors tensors anywhere in memory, all of `type`, in place (optim.AdamW; upstream
  * has Adam only).  All pointers in the arrays are DEVICE, the arrays themselves and counts HOST.  Tensor i: counts[i] elements

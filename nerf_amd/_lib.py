@@ -101,6 +101,10 @@ SIGNATURES = {
     "nerf_fp8_quantize": (_i, [_l, _l, _i, _p, _l, _p, _l, _p, _p, _p, _p, _i, _p, _p, _p]),
     "nerf_fp8_matmul_workspace_floats": (_l, [_l, _l, _l, _i]),
     "nerf_fp8_matmul": (_i, [_l, _l, _l, _p, _p, _p, _p, _i, _p, _i, _i, _p, _l, _p, _p]),
+    "nerf_linear_fp8_kept_bytes": (_l, [_l, _l, _l, _i, _i]),
+    "nerf_linear_fp8_workspace_bytes": (_l, [_l, _l, _l, _i, _i, _i]),
+    "nerf_linear_fp8_fwd": (_i, [_l, _l, _l, _i, _p, _l, _i, _p, _l, _p, _p, _i, _p, _i, _p, _p, _i, _i, _p, _p]),
+    "nerf_linear_fp8_bwd": (_i, [_l, _l, _l, _i, _p, _l, _p, _p, _i, _i, _p, _i, _p, _i, _p, _p, _p]),
     "nerf_adamw_workspace_floats": (_l, [_i]),
     "nerf_adamw_step": (_i, [_i, _p, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p, _d, _d, _d, _d, _d, _p, _p]),
     "nerf_mlp_bwd_static_max_points": (_l, []),

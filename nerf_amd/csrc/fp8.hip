@@ -780,4 +780,95 @@ int64_t nerf_fp8_matmul_workspace_floats(int64_t m, int64_t n, int64_t k, int ty
     return plan.slices > 1 ? plan.slices * m * n : 0;
 }
 
+// What a layer keeps for its backward pass and needs for a while, as offsets of 256 bytes' multiples into two buffers.
+namespace {
+inline int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
+struct Held {      // a quantised matrix [rows, k] inside a buffer
+    int64_t codes, scales, end;
+    Held(int64_t at, int64_t rows, int64_t k) : codes(at), scales(at + up256(rows * code_stride(k))), end(scales + up256(rows * scale_stride(k))) {}
+};
+struct Kept {
+    Held xt, wt;      // x^T [n_in, n], w^T [n_in, n_out]
+    Kept(int64_t n, int64_t n_in, int64_t n_out, bool dx, bool dw) : xt(0, dw ? n_in : 0, n), wt(xt.end, dx ? n_in : 0, n_out) {}
+};
+struct Forward {
+    Held x, w;
+    int64_t part, end;
+    Forward(int64_t n, int64_t n_in, int64_t n_out, int type)
+        : x(0, n, n_in), w(x.end, n_out, n_in), part(w.end), end(part + up256(4 * nerf_fp8_matmul_workspace_floats(n, n_out, n_in, type))) {}
+};
+struct Backward {
+    Held g, gt;       // dy [n, n_out], dy^T [n_out, n]
+    int64_t sums, part, end;
+    Backward(int64_t n, int64_t n_in, int64_t n_out, int type, int w_type)
+        : g(0, n, n_out), gt(g.end, n_out, n), sums(gt.end), part(sums + up256(4 * nerf_fp8_quantize_workspace_floats(n, n_out))), end(part) {
+        const int64_t a = nerf_fp8_matmul_workspace_floats(n, n_in, n_out, type), b = nerf_fp8_matmul_workspace_floats(n_out, n_in, n, w_type);
+        end += up256(4 * (a > b ? a : b));      // (one product after the other)
+    }
+};
+}  // namespace
+
+int64_t nerf_linear_fp8_kept_bytes(int64_t n, int64_t n_in, int64_t n_out, int needs_dx, int needs_dw) {
+    return n < 1 || n_in < 1 || n_out < 1 ? 0 : Kept(n, n_in, n_out, needs_dx != 0, needs_dw != 0).wt.end;
+}
+int64_t nerf_linear_fp8_workspace_bytes(int64_t n, int64_t n_in, int64_t n_out, int type, int w_type, int backward) {
+    if (n < 1 || n_in < 1 || n_out < 1) return 0;
+    return backward ? Backward(n, n_in, n_out, type, w_type).end : Forward(n, n_in, n_out, type).end;
+}
+
+int nerf_linear_fp8_fwd(int64_t n, int64_t n_in, int64_t n_out, int type, const void* x, int64_t ldx, int w_type, const void* w, int64_t ldw,
+                        const uint8_t* w_codes, const uint8_t* w_scales, int bias_type, const void* bias, int relu, void* y, void* kept,
+                        int needs_dx, int needs_dw, void* workspace, void* stream) {
+    NERF_REQUIRE(n >= 0 && n_in >= 1 && n_out >= 1, "nerf_linear_fp8_fwd: n=%lld n_in=%lld n_out=%lld", (long long)n, (long long)n_in, (long long)n_out);
+    NERF_REQUIRE(elem_type_ok(type) && (!w || w_type == type || w_type == NERF_F32), "nerf_linear_fp8_fwd: type=%d w_type=%d", type, w_type);
+    if (n == 0) return 0;
+    NERF_REQUIRE(x && y && workspace && (w || (w_codes && w_scales && !kept)), "nerf_linear_fp8_fwd: null pointer");
+    NERF_REQUIRE(((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(kept)) & 255) == 0,
+                 "nerf_linear_fp8_fwd: kept and workspace start at a multiple of 256 bytes");
+    uint8_t* ws = (uint8_t*)workspace;
+    uint8_t* keep = (uint8_t*)kept;
+    const Forward f(n, n_in, n_out, type);
+    const bool kx = keep && needs_dw, kw = keep && needs_dx;
+    const Kept k(n, n_in, n_out, kw, kx);
+    int rc = nerf_fp8_quantize(n, n_in, type, x, ldx, nullptr, 0, ws + f.x.codes, ws + f.x.scales, kx ? keep + k.xt.codes : nullptr,
+                               kx ? keep + k.xt.scales : nullptr, NERF_F32, nullptr, nullptr, stream);
+    if (rc) return rc;
+    if (w) {
+        rc = nerf_fp8_quantize(n_out, n_in, w_type, w, ldw, nullptr, 0, ws + f.w.codes, ws + f.w.scales, kw ? keep + k.wt.codes : nullptr,
+                               kw ? keep + k.wt.scales : nullptr, NERF_F32, nullptr, nullptr, stream);
+        if (rc) return rc;
+        w_codes = ws + f.w.codes;
+        w_scales = ws + f.w.scales;
+    }
+    return nerf_fp8_matmul(n, n_out, n_in, ws + f.x.codes, ws + f.x.scales, w_codes, w_scales, bias_type, bias, relu, type, y, n_out,
+                           (float*)(ws + f.part), stream);
+}
+
+int nerf_linear_fp8_bwd(int64_t n, int64_t n_in, int64_t n_out, int type, const void* dy, int64_t lddy, const void* y, const void* kept,
+                        int needs_dx, int needs_dw, void* dx, int w_type, void* dw, int bias_type, void* db, void* workspace, void* stream) {
+    NERF_REQUIRE(n >= 1 && n_in >= 1 && n_out >= 1, "nerf_linear_fp8_bwd: n=%lld n_in=%lld n_out=%lld", (long long)n, (long long)n_in, (long long)n_out);
+    NERF_REQUIRE(elem_type_ok(type) && (w_type == type || w_type == NERF_F32) && (!db || bias_type == type || bias_type == NERF_F32),
+                 "nerf_linear_fp8_bwd: type=%d w_type=%d bias_type=%d", type, w_type, bias_type);
+    if (!dx && !dw && !db) return 0;
+    NERF_REQUIRE(dy && workspace && ((!dx && !dw) || kept), "nerf_linear_fp8_bwd: null pointer");
+    NERF_REQUIRE((!dx || needs_dx) && (!dw || needs_dw), "nerf_linear_fp8_bwd: a gradient is asked for that the forward pass kept nothing for");
+    NERF_REQUIRE(((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(kept)) & 255) == 0,
+                 "nerf_linear_fp8_bwd: kept and workspace start at a multiple of 256 bytes");
+    uint8_t* ws = (uint8_t*)workspace;
+    const uint8_t* keep = (const uint8_t*)kept;
+    const Backward b(n, n_in, n_out, type, w_type);
+    const Kept k(n, n_in, n_out, needs_dx != 0, needs_dw != 0);
+    int rc = nerf_fp8_quantize(n, n_out, type, dy, lddy, y, n_out, dx ? ws + b.g.codes : nullptr, dx ? ws + b.g.scales : nullptr,
+                               dw ? ws + b.gt.codes : nullptr, dw ? ws + b.gt.scales : nullptr, bias_type, db, (float*)(ws + b.sums), stream);
+    if (rc) return rc;
+    if (dx) {
+        rc = nerf_fp8_matmul(n, n_in, n_out, ws + b.g.codes, ws + b.g.scales, keep + k.wt.codes, keep + k.wt.scales, type, nullptr, 0, type, dx, n_in,
+                             (float*)(ws + b.part), stream);
+        if (rc) return rc;
+    }
+    if (!dw) return 0;
+    return nerf_fp8_matmul(n_out, n_in, n, ws + b.gt.codes, ws + b.gt.scales, keep + k.xt.codes, keep + k.xt.scales, w_type, nullptr, 0, w_type, dw, n_in,
+                           (float*)(ws + b.part), stream);
+}
+
 }  // extern "C"

@@ -941,6 +941,31 @@ def _vector(t: Optional[torch.Tensor], size: int, like: torch.Tensor, what: str)
     return t.contiguous()
 
 
+# A launch on the tensors' device and its current stream, bracketed with events when PROFILE is a list.  (Torch's device context and
+# stream objects cost several microseconds each, which a call of a few microseconds would spend twice over.)
+def _launch(dev: torch.device, name: str, units: int, fn, *args) -> None:
+    if dev.index == torch.cuda.current_device():
+        if PROFILE is None:
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+            if rc:
+                check(rc)
+            return
+        with _timed(name, units):
+            check(fn(*args, _stream()))
+        return
+    with torch.cuda.device(dev), _timed(name, units):
+        check(fn(*args, _stream()))
+
+
+def _differentiable_once(backward):
+    """torch.autograd.function.once_differentiable, paid for only where a graph of the backward pass is asked for."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 class _LayerNorm(torch.autograd.Function):
     """Layer norm over the last dimension, forward and backward in libnerf_hip.so (layer_norm.hip)."""
 
@@ -948,37 +973,35 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, w, b, eps, need_grad):
         x2 = _rows_any(x, "x")
         n, c = x2.shape
+        dev, dtype = x2.device, x2.dtype
         wc, bc = _vector(w, c, x2, "weight"), _vector(b, c, x2, "bias")
-        if wc is not None and bc is not None and wc.dtype != bc.dtype:
+        w_dtype = dtype if wc is None and bc is None else (bc if wc is None else wc).dtype
+        if wc is not None and bc is not None and bc.dtype != w_dtype:
             raise TypeError(f"layer_norm: weight is {wc.dtype}, bias {bc.dtype}")
-        w_type = _elem(wc if wc is not None else bc if bc is not None else x2, "weight")
-        y = torch.empty((n, c), dtype=x.dtype, device=x2.device)
-        stats = torch.empty((3, n), dtype=torch.float32, device=x2.device) if need_grad else None
-        with torch.cuda.device(x2.device), _timed("layer_norm", 2 * n * c * x2.element_size()):
-            check(lib.nerf_layer_norm_fwd(n, c, ELEM_TYPES[x2.dtype], x2.data_ptr(), _ld(x2), w_type, _ptr(wc), _ptr(bc), eps,
-                                          y.data_ptr(), c, _ptr(stats), _stream()))
-        ctx.save_for_backward(x2, wc, stats)
-        ctx.lead, ctx.w_type = tuple(x.shape[:-1]), w_type
-        return y.reshape(ctx.lead + (c,))
+        y = torch.empty(x.shape, dtype=dtype, device=dev)
+        stats = torch.empty((3, n), dtype=torch.float32, device=dev) if need_grad else None
+        _launch(dev, "layer_norm", 2 * n * c * x2.element_size(), lib.nerf_layer_norm_fwd, n, c, ELEM_TYPES[dtype], x2.data_ptr(), _ld(x2),
+                ELEM_TYPES[w_dtype], _ptr(wc), _ptr(bc), eps, y.data_ptr(), c, _ptr(stats))
+        if need_grad:
+            ctx.save_for_backward(x2, wc, stats)
+            ctx.w_dtype = w_dtype
+        return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiable_once
     def backward(ctx, dy):
         x2, wc, stats = ctx.saved_tensors
         n, c = x2.shape
+        dev, dtype, w_dtype = x2.device, x2.dtype, ctx.w_dtype
         dy2 = _rows_any(dy, "grad")
-        dev = x2.device
-        w_dtype = {v: k for k, v in ELEM_TYPES.items()}[ctx.w_type]
-        dx = torch.empty((n, c), dtype=x2.dtype, device=dev) if ctx.needs_input_grad[0] else None
-        dw = torch.empty((c,), dtype=w_dtype, device=dev) if ctx.needs_input_grad[1] else None
-        db = torch.empty((c,), dtype=w_dtype, device=dev) if ctx.needs_input_grad[2] else None
-        ws = None
-        if dw is not None or db is not None:
-            ws = torch.empty(lib.nerf_layer_norm_workspace_floats(n, c), dtype=torch.float32, device=dev)
-        with torch.cuda.device(dev), _timed("layer_norm_bwd", 3 * n * c * x2.element_size()):
-            check(lib.nerf_layer_norm_bwd(n, c, ELEM_TYPES[x2.dtype], x2.data_ptr(), _ld(x2), dy2.data_ptr(), _ld(dy2), ctx.w_type,
-                                          _ptr(wc), _ptr(stats), _ptr(dx), c, _ptr(dw), _ptr(db), _ptr(ws), _stream()))
-        return None if dx is None else dx.reshape(ctx.lead + (c,)), dw, db, None, None
+        need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
+        dx = torch.empty(dy.shape, dtype=dtype, device=dev) if need_dx else None
+        dw = torch.empty((c,), dtype=w_dtype, device=dev) if need_dw else None
+        db = torch.empty((c,), dtype=w_dtype, device=dev) if need_db else None
+        ws = torch.empty((lib.nerf_layer_norm_workspace_floats(n, c),), dtype=torch.float32, device=dev) if need_dw or need_db else None
+        _launch(dev, "layer_norm_bwd", 3 * n * c * x2.element_size(), lib.nerf_layer_norm_bwd, n, c, ELEM_TYPES[dtype], x2.data_ptr(), _ld(x2),
+                dy2.data_ptr(), _ld(dy2), ELEM_TYPES[w_dtype], _ptr(wc), stats.data_ptr(), _ptr(dx), c, _ptr(dw), _ptr(db), _ptr(ws))
+        return dx, dw, db, None, None
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -1034,10 +1057,9 @@ def _quantize(x2: torch.Tensor, want: bool, want_t: bool, mask: Optional[torch.T
     if sum_dtype is not None:
         sums = torch.empty((cols,), dtype=sum_dtype, device=dev)
         ws = torch.empty(lib.nerf_fp8_quantize_workspace_floats(rows, cols), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev), _timed("fp8_quantize", rows * cols * (x2.element_size() + int(want) + int(want_t))):
-        check(lib.nerf_fp8_quantize(rows, cols, ELEM_TYPES[x2.dtype], x2.data_ptr(), _ld(x2), _ptr(mask), 0 if mask is None else _ld(mask),
-                                    _ptr(q[0]), _ptr(q[1]), _ptr(qt[0]), _ptr(qt[1]), 0 if sums is None else ELEM_TYPES[sum_dtype],
-                                    _ptr(sums), _ptr(ws), _stream()))
+    _launch(dev, "fp8_quantize", rows * cols * (x2.element_size() + int(want) + int(want_t)), lib.nerf_fp8_quantize, rows, cols,
+            ELEM_TYPES[x2.dtype], x2.data_ptr(), _ld(x2), _ptr(mask), 0 if mask is None else _ld(mask), _ptr(q[0]), _ptr(q[1]), _ptr(qt[0]),
+            _ptr(qt[1]), 0 if sums is None else ELEM_TYPES[sum_dtype], _ptr(sums), _ptr(ws))
     return Fp8Rows(*q, cols) if want else None, Fp8Rows(*qt, rows) if want_t else None, sums
 
 
@@ -1067,11 +1089,31 @@ def matmul_fp8(a: Fp8Rows, b: Fp8Rows, bias: Optional[torch.Tensor] = None, relu
     kind = ELEM_TYPES[out_dtype]
     floats = lib.nerf_fp8_matmul_workspace_floats(a.rows, b.rows, a.k, kind)
     ws = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
-    with torch.cuda.device(dev), _timed("fp8_matmul", 2 * a.rows * b.rows * a.k):
-        check(lib.nerf_fp8_matmul(a.rows, b.rows, a.k, a.codes.data_ptr(), a.scales.data_ptr(), b.codes.data_ptr(), b.scales.data_ptr(),
-                                  kind if bias is None else ELEM_TYPES[bias.dtype], _ptr(bias), int(bool(relu)), kind, c.data_ptr(),
-                                  b.rows, _ptr(ws), _stream()))
+    _launch(dev, "fp8_matmul", 2 * a.rows * b.rows * a.k, lib.nerf_fp8_matmul, a.rows, b.rows, a.k, a.codes.data_ptr(), a.scales.data_ptr(),
+            b.codes.data_ptr(), b.scales.data_ptr(), kind if bias is None else ELEM_TYPES[bias.dtype], _ptr(bias), int(bool(relu)), kind,
+            c.data_ptr(), b.rows, _ptr(ws))
     return c
+
+
+def _bytes(count: int, dev) -> Optional[torch.Tensor]:
+    return torch.empty((count,), dtype=torch.uint8, device=dev) if count else None
+
+
+def _linear_fp8_forward(x: torch.Tensor, x2: torch.Tensor, w2, n_out: int, b, relu: bool, need_dx: bool, need_dw: bool):
+    """-> (y, what the backward pass needs of x and w in 8 bits); w2: a matrix of rows, or an Fp8Rows."""
+    n, n_in = x2.shape
+    dev, kind = x2.device, ELEM_TYPES[x2.dtype]
+    bias = _vector(b, n_out, x2, "bias")
+    y = torch.empty(x.shape[:-1] + (n_out,), dtype=x2.dtype, device=dev)
+    kept = _bytes(lib.nerf_linear_fp8_kept_bytes(n, n_in, n_out, need_dx, need_dw), dev) if need_dx or need_dw else None
+    ws = _bytes(lib.nerf_linear_fp8_workspace_bytes(n, n_in, n_out, kind, 0, 0), dev)
+    if isinstance(w2, Fp8Rows):
+        weight = (0, None, 0, w2.codes.data_ptr(), w2.scales.data_ptr())
+    else:
+        weight = (ELEM_TYPES[w2.dtype], w2.data_ptr(), _ld(w2), None, None)
+    _launch(dev, "linear_fp8", 2 * n * n_in * n_out, lib.nerf_linear_fp8_fwd, n, n_in, n_out, kind, x2.data_ptr(), _ld(x2), *weight,
+            kind if bias is None else ELEM_TYPES[bias.dtype], _ptr(bias), int(relu), y.data_ptr(), _ptr(kept), need_dx, need_dw, _ptr(ws))
+    return y, kept
 
 
 class _LinearFp8(torch.autograd.Function):
@@ -1082,37 +1124,33 @@ class _LinearFp8(torch.autograd.Function):
     def forward(ctx, x, w, b, relu, need_grad):
         x2, w2 = _rows_any(x, "x"), _rows_any(w, "weight")
         need_dx, need_dw = need_grad and ctx.needs_input_grad[0], need_grad and ctx.needs_input_grad[1]
-        xq, xt, _ = _quantize(x2, True, need_dw and x2.shape[0] > 0)
-        wq, wt, _ = _quantize(w2, True, need_dx)
-        y = matmul_fp8(xq, wq, b, relu, x2.dtype)
-        kept = [t for q in (xt, wt) if q is not None for t in (q.codes, q.scales)]
-        ctx.save_for_backward(*kept, *([y] if relu and need_grad else []))
-        ctx.kept = xt is not None, wt is not None, bool(relu)
-        ctx.lead, ctx.shape, ctx.w_dtype, ctx.b_dtype = tuple(x.shape[:-1]), (x2.shape[0],) + tuple(w2.shape), w.dtype, None if b is None else b.dtype
-        return y.reshape(ctx.lead + (w2.shape[0],))
+        n_out, n_in = w2.shape
+        y, kept = _linear_fp8_forward(x, x2, w2, n_out, b, relu, need_dx, need_dw)
+        if need_grad:
+            ctx.save_for_backward(kept, y if relu else None)
+            ctx.args = (x2.shape[0], n_in, n_out, need_dx, need_dw, w.dtype, None if b is None else b.dtype)
+        return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiable_once
     def backward(ctx, dy):
-        saved = list(ctx.saved_tensors)
-        n, n_out, n_in = ctx.shape
-        xt = Fp8Rows(saved.pop(0), saved.pop(0), n) if ctx.kept[0] else None
-        wt = Fp8Rows(saved.pop(0), saved.pop(0), n_out) if ctx.kept[1] else None
-        y = saved.pop(0) if ctx.kept[2] else None
-        dy2 = _rows_any(dy, "grad")
+        kept, y = ctx.saved_tensors
+        n, n_in, n_out, kept_dx, kept_dw, w_dtype, b_dtype = ctx.args
         need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
-        dx = dw = db = None
+        dy2 = _rows_any(dy, "grad")
+        dev, kind = dy2.device, ELEM_TYPES[dy2.dtype]
+        dx = torch.empty(dy.shape[:-1] + (n_in,), dtype=dy2.dtype, device=dev) if need_dx else None
         if n == 0:
-            dx = torch.empty((0, n_in), dtype=dy.dtype, device=dy.device) if need_dx else None
-            dw = torch.zeros((n_out, n_in), dtype=ctx.w_dtype, device=dy.device) if need_dw else None
-            db = torch.zeros((n_out,), dtype=ctx.b_dtype, device=dy.device) if need_db else None
-        elif need_dx or need_dw or need_db:
-            gq, gt, db = _quantize(dy2, need_dx, need_dw, y, ctx.b_dtype if need_db else None)
-            if need_dx:
-                dx = matmul_fp8(gq, wt, out_dtype=dy2.dtype)
-            if need_dw:
-                dw = matmul_fp8(gt, xt, out_dtype=ctx.w_dtype)
-        return None if dx is None else dx.reshape(ctx.lead + (n_in,)), dw, db, None, None
+            dw = torch.zeros((n_out, n_in), dtype=w_dtype, device=dev) if need_dw else None
+            db = torch.zeros((n_out,), dtype=b_dtype, device=dev) if need_db else None
+            return dx, dw, db, None, None
+        dw = torch.empty((n_out, n_in), dtype=w_dtype, device=dev) if need_dw else None
+        db = torch.empty((n_out,), dtype=b_dtype, device=dev) if need_db else None
+        ws = _bytes(lib.nerf_linear_fp8_workspace_bytes(n, n_in, n_out, kind, ELEM_TYPES[w_dtype], 1), dev)
+        _launch(dev, "linear_fp8_bwd", 4 * n * n_in * n_out, lib.nerf_linear_fp8_bwd, n, n_in, n_out, kind, dy2.data_ptr(), _ld(dy2), _ptr(y),
+                _ptr(kept), kept_dx, kept_dw, _ptr(dx), ELEM_TYPES[w_dtype], _ptr(dw), 0 if db is None else ELEM_TYPES[b_dtype], _ptr(db),
+                ws.data_ptr())
+        return dx, dw, db, None, None
 
 
 def linear_fp8(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = None, relu: bool = False) -> torch.Tensor:
@@ -1126,12 +1164,13 @@ def linear_fp8(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = None, rel
         x2 = _rows_any(x, "x")
         if x2.shape[1] != weight.k:
             raise ValueError(f"linear_fp8: x has {x2.shape[1]} values per row, the weight k={weight.k}")
-        y = matmul_fp8(_quantize(x2, True, False)[0], weight, bias, relu, x2.dtype)
-        return y.reshape(tuple(x.shape[:-1]) + (weight.rows,))
+        if weight.codes.device != x2.device:
+            raise TypeError(f"linear_fp8: x on {x2.device}, the weight on {weight.codes.device}")
+        return _linear_fp8_forward(x, x2, weight, weight.rows, bias, bool(relu), False, False)[0]
     _elem(x, "x")
     if weight.dim() != 2 or x.dim() < 1 or weight.shape[1] != x.shape[-1]:
         raise ValueError(f"linear_fp8: x {tuple(x.shape)} against weight {tuple(weight.shape)}")
     if weight.device != x.device or weight.dtype not in (x.dtype, torch.float32):
         raise TypeError(f"linear_fp8: expected a weight in {x.dtype} or fp32 on {x.device}, got {weight.dtype} on {weight.device}")
     need = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias))
-    return _LinearFp8.apply(x, weight, bias, relu, need)
+    return _LinearFp8.apply(x, weight, bias, bool(relu), need)

@@ -20,12 +20,16 @@ moments into their buffers and reads one word back from the device.
 from __future__ import annotations
 
 import ctypes
+import itertools
+import operator
+from array import array
 from typing import List, Optional
 
 import torch
 
 from ._lib import check, lib
 from .ops import ELEM_TYPES
+from .ops import _launch as _launch_on
 
 
 class _Run:
@@ -204,6 +208,82 @@ class FlatAdam(torch.optim.Adam):
         self._layout_key = None
 
 
+def _address(values: array) -> int:
+    return values.buffer_info()[0]
+
+
+_data_ptr, _numel, _is_contiguous, _get_device = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device
+
+
+class _Launch:
+    """The tensors of a group that share a device and a type, as the kernel takes them: host arrays of addresses and counts."""
+    __slots__ = ("device", "dtype", "kind", "index", "params", "counts", "devices", "pointers", "bytes")
+
+    def __init__(self, device, dtype, index, params, states):
+        self.device, self.dtype, self.kind = device, dtype, ELEM_TYPES[dtype]
+        self.index, self.params = index, params
+        self.devices = array("q", [device.index] * len(index))
+        self.counts = array("q", map(_numel, params))
+        self.pointers = {"params": array("Q", map(_data_ptr, params))}
+        self.bytes = 0
+        for name in ("exp_avg", "exp_avg_sq", "scale", "master", "step"):
+            ts = [st.get(name) for st in states]
+            self.pointers[name] = array("Q", [0 if t is None else t.data_ptr() for t in ts])
+            self.bytes += sum(0 if t is None else 2 * t.numel() * t.element_size() for t in ts)
+        self.bytes += 3 * sum(self.counts) * dtype.itemsize
+
+    def take(self, all_grads):
+        """This step's gradients: (addresses, the tensors they belong to)."""
+        grads = [all_grads[i] for i in self.index]
+        if not all(g.layout is torch.strided for g in grads):
+            raise TypeError("AdamW: sparse gradients are not supported")
+        if not all(g.dtype is self.dtype for g in grads) or array("q", map(_get_device, grads)) != self.devices:
+            raise TypeError(f"AdamW: a gradient is not in {self.dtype} on {self.device}, as its parameter is")
+        if array("q", map(_numel, grads)) != self.counts:
+            raise ValueError("AdamW: a gradient has another size than its parameter")
+        if not all(map(_is_contiguous, grads)):
+            grads = [g.contiguous() for g in grads]
+        return array("Q", map(_data_ptr, grads)), grads
+
+
+class _Plan:
+    """What a step of a group needs to know and seldom changes: which tensors take part, their states and addresses.  Every step
+    looks whether it still stands -- the same tensor objects, at the same addresses, of the same sizes --, with a few passes over lists
+    instead of a dozen checks per tensor (for 48 small tensors those cost more than the launch)."""
+    __slots__ = ("params", "absent", "states", "held", "pointed", "addresses", "live", "counts", "launches")
+
+    def __init__(self, opt, params, grads):
+        self.params, self.absent = list(params), [g is None for g in grads]
+        lists = {}
+        for i, (p, g) in enumerate(zip(params, grads)):
+            if g is None:
+                continue
+            if g.layout != torch.strided:
+                raise TypeError("AdamW: sparse gradients are not supported")
+            if p.dtype not in ELEM_TYPES or not p.is_cuda:
+                raise TypeError(f"AdamW: expected fp32, bf16 or fp16 parameters on a HIP device, got {p.dtype} on {p.device}")
+            if not p.is_contiguous():
+                raise ValueError(f"AdamW: a parameter of shape {tuple(p.shape)} is not contiguous")
+            lists.setdefault((p.device, p.dtype), []).append(i)
+        self.live = [p for p, none in zip(params, self.absent) if not none]
+        self.states = [opt._checked_state(p) for p in self.live]
+        state_of = dict(zip(map(id, self.live), self.states))
+        self.held = list(itertools.chain.from_iterable(map(dict.values, self.states)))
+        self.pointed = self.live + [t for t in self.held if torch.is_tensor(t)]
+        self.addresses = array("Q", map(_data_ptr, self.pointed))
+        self.counts = array("q", map(_numel, self.live))
+        self.launches = [_Launch(device, dtype, index, [params[i] for i in index], [state_of[id(params[i])] for i in index])
+                         for (device, dtype), index in lists.items()]
+
+    def stands(self, params, grads) -> bool:
+        if len(params) != len(self.params) or not all(map(operator.is_, params, self.params)) or [g is None for g in grads] != self.absent:
+            return False
+        held = list(itertools.chain.from_iterable(map(dict.values, self.states)))
+        return (len(held) == len(self.held) and all(map(operator.is_, held, self.held))
+                and array("Q", map(_data_ptr, self.pointed)) == self.addresses and array("q", map(_numel, self.live)) == self.counts
+                and all(map(_is_contiguous, self.live)))
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay) over any tensors, wherever they lie: one launch of the library's kernel per 60 tensors of a
     group, device and type, after a small one that counts the steps -- where FlatAdam needs parameters and gradients back to back.
@@ -226,7 +306,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: state_bits={state_bits} is neither 32 nor 8")
         self._check_hyper(lr, betas, eps, weight_decay)
         self.state_bits = state_bits
-        self._slots = {}      # parameter -> (its state dict, the dict's tensors, their addresses): see _slot
+        self._plans, self._seen = {}, []      # what the last step looked up: see _Plan
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, capturable=True))
 
     @staticmethod
@@ -267,8 +347,8 @@ class AdamW(torch.optim.Optimizer):
                 out[name] = torch.zeros(shape, dtype=dtype, device=p.device)
         return out
 
-    def _slot(self, p):
-        """The state's addresses, checked when a state is first seen: (dict, its tensors, exp_avg, exp_avg_sq, scale, master, step)."""
+    def _checked_state(self, p):
+        """The state of `p` -- made on first use --, which the kernel will read by address: every tensor of the layout it assumes."""
         st = self.state[p]
         if not st:
             if torch.cuda.is_current_stream_capturing():
@@ -276,25 +356,10 @@ class AdamW(torch.optim.Optimizer):
             st.update(self._new_state(p))
         for name, (dtype, shape) in self._layout(p).items():
             t = st.get(name)
-            if (not torch.is_tensor(t) or t.dtype != dtype or t.shape != shape or t.device != p.device or not t.is_contiguous()):
+            if not torch.is_tensor(t) or t.dtype != dtype or t.shape != shape or t.device != p.device or not t.is_contiguous():
                 raise ValueError(f"AdamW: the state's {name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {p.device}, got "
                                  f"{(t.dtype, tuple(t.shape), t.device) if torch.is_tensor(t) else t}")
-        names = ("exp_avg", "exp_avg_sq", "scale", "master", "step")
-        tensors = tuple(st.get(name) for name in names)
-        slot = (st, tensors, tuple(0 if t is None else t.data_ptr() for t in tensors), p.shape, p.dtype, p.device)
-        self._slots[p] = slot
-        return slot
-
-    def _current(self, p):
-        """The slot of `p`, made anew when its state or the parameter itself is no longer the one seen before."""
-        slot = self._slots.get(p)
-        if slot is not None:
-            st, (m, v, scale, master, step), _, shape, dtype, device = slot
-            if (self.state.get(p) is st and st.get("exp_avg") is m and st.get("exp_avg_sq") is v and st.get("step") is step
-                    and st.get("scale") is scale and st.get("master") is master
-                    and p.dtype is dtype and p.shape == shape and p.device == device):
-                return slot
-        return self._slot(p)
+        return st
 
     # ---- the step ------------------------------------------------------------------------------------
     @torch.no_grad()
@@ -303,48 +368,35 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        states = list(self.state.values())
+        known = len(states) == len(self._seen) and all(map(operator.is_, states, self._seen))
         work = []
-        for group in self.param_groups:
-            lists = {}      # (device, type) -> rows of (count, p, g, exp_avg, exp_avg_sq, scale, master, step)
-            for p in group["params"]:
-                g = p.grad
-                if g is None:
-                    continue
-                if g.is_sparse or g.layout != torch.strided:
-                    raise TypeError("AdamW: sparse gradients are not supported")
-                if p.dtype not in ELEM_TYPES or not p.is_cuda:
-                    raise TypeError(f"AdamW: expected fp32, bf16 or fp16 parameters on a HIP device, got {p.dtype} on {p.device}")
-                if not p.is_contiguous():
-                    raise ValueError(f"AdamW: a parameter of shape {tuple(p.shape)} is not contiguous")
-                if g.dtype != p.dtype or g.device != p.device:
-                    raise TypeError(f"AdamW: a gradient in {g.dtype} on {g.device} for a parameter in {p.dtype} on {p.device}")
-                if not g.is_contiguous():
-                    g = g.contiguous()
-                lists.setdefault((p.device, p.dtype), []).append((p, g, self._current(p)))
-            work.append((group, lists))
-        for group, lists in work:
+        for group in self.param_groups:      # (everything is checked before anything is launched)
             self._check_hyper(group["lr"], group["betas"], group["eps"], group["weight_decay"])
-            for (device, dtype), rows in lists.items():
-                self._launch(group, device, dtype, rows)
+            grads = [p.grad for p in group["params"]]
+            plan = self._plans.get(id(group)) if known else None
+            if plan is None or not plan.stands(group["params"], grads):
+                plan = self._plans[id(group)] = _Plan(self, group["params"], grads)
+            work += [(group, launch, launch.take(grads)) for launch in plan.launches]
+        self._seen = list(self.state.values())
+        for group, launch, (addresses, _) in work:
+            self._launch(group, launch, addresses)
         return loss
 
-    def _launch(self, group, device, dtype, rows):
-        n = len(rows)
-        lr, lr_dev = group["lr"], None
+    def _launch(self, group, launch, grads):
+        device, lr, lr_dev = launch.device, group["lr"], None
         if torch.is_tensor(lr) and lr.is_cuda:
             if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != device:
                 raise TypeError(f"AdamW: a device learning rate must be one fp32 value on {device}, got {lr.dtype} on {lr.device}")
             lr_dev, lr = lr.data_ptr(), 0.0
-        pointers = ctypes.c_void_p * n
-        counts = (ctypes.c_int64 * n)(*[p.numel() for p, _, _ in rows])
-        params = pointers(*[p.data_ptr() for p, _, _ in rows])
-        grads = pointers(*[g.data_ptr() for _, g, _ in rows])
-        m, v, scale, master, step = [pointers(*column) for column in zip(*[slot[2] for _, _, slot in rows])]
-        with torch.cuda.device(device):
-            coef = torch.empty(lib.nerf_adamw_workspace_floats(n), dtype=torch.float32, device=device)
-            check(lib.nerf_adamw_step(n, counts, ELEM_TYPES[dtype], self.state_bits, params, grads, m, v, scale, master, step, lr_dev,
-                                      float(lr), float(group["betas"][0]), float(group["betas"][1]), float(group["eps"]),
-                                      float(group["weight_decay"]), coef.data_ptr(), torch.cuda.current_stream().cuda_stream))
+        n = len(launch.params)
+        coef = torch.empty((4 * n,), dtype=torch.float32, device=device)
+        beta1, beta2 = group["betas"]
+        _launch_on(device, "adamw", launch.bytes, lib.nerf_adamw_step, n, _address(launch.counts), launch.kind, self.state_bits,
+                   _address(launch.pointers["params"]), _address(grads), _address(launch.pointers["exp_avg"]),
+                   _address(launch.pointers["exp_avg_sq"]), _address(launch.pointers["scale"]), _address(launch.pointers["master"]),
+                   _address(launch.pointers["step"]), lr_dev, float(lr), float(beta1), float(beta2), float(group["eps"]),
+                   float(group["weight_decay"]), coef.data_ptr())
 
     # ---- checkpoints ---------------------------------------------------------------------------------
     def load_state_dict(self, state_dict):
@@ -373,7 +425,7 @@ class AdamW(torch.optim.Optimizer):
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         for group in self.param_groups:
             group["capturable"] = True
-        self._slots = {}
+        self._plans, self._seen = {}, []
         for p, new in fresh.items():
             self.state[p] = new
 
@@ -382,4 +434,4 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._slots = {}
+        self._plans, self._seen = {}, []

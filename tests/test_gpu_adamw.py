@@ -356,6 +356,52 @@ def test_graphs_and_streams(device, bits):
             fresh.step()
 
 
+def test_tensors_exchanged_between_steps(device):
+    """Whatever is swapped between two steps is seen by the next: gradients that come and go, a parameter's storage, a state's tensor
+    or storage, a whole state, the group's list."""
+    params = _params([(300,), (40, 30), (700,), (5,)], torch.float32, device, 21)
+    opt = _opt(params)
+    for t in (1, 2):
+        _step_and_check(opt, params, t)
+    for p in params:                        # as zero_grad() and a backward pass would
+        p.grad = torch.randn_like(p)
+    _step_and_check(opt, params, 3)
+    params[0].data = params[0].data.clone()
+    _step_and_check(opt, params, 4)
+    st = opt.state[params[1]]
+    st["exp_avg"] = st["exp_avg"].clone()
+    st["exp_avg_sq"].data = st["exp_avg_sq"].data.clone()
+    _step_and_check(opt, params, 5)
+    opt.state[params[2]] = {k: v.clone() for k, v in opt.state[params[2]].items()}
+    _step_and_check(opt, params, 6)
+    late, params[3].grad = params[3].grad, None
+    _step_and_check(opt, params[:3], 7)
+    params[3].grad = late
+    assert float(opt.state[params[3]]["step"]) == 6.0
+    opt.step()
+    assert [float(opt.state[p]["step"]) for p in params] == [8.0, 8.0, 8.0, 7.0]
+    extra = _params([(64,)], torch.float32, device, 22)
+    opt.add_param_group({"params": extra, "lr": 1e-4})
+    opt.step()
+    assert float(opt.state[extra[0]]["step"]) == 1.0 and float(opt.state[params[0]]["step"]) == 9.0
+    opt.state.clear()
+    opt.step()
+    assert float(opt.state[params[0]]["step"]) == 1.0
+
+
+def test_a_size_that_no_longer_fits_is_refused(device):
+    p = _params([(300,)], torch.float32, device, 23)[0]
+    opt = _opt([p])
+    opt.step()
+    before = p.data.clone()
+    p.data = p.data[:10]
+    with pytest.raises(ValueError):
+        opt.step()
+    p.data = before.to("cpu")
+    with pytest.raises((TypeError, ValueError)):
+        opt.step()
+
+
 def test_refusals(device):
     from nerf_amd.optim import AdamW
     p = _params([(8, 6)], torch.float32, device, 11)[0]

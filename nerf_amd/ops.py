@@ -919,26 +919,30 @@ def _elem(t: torch.Tensor, what: str) -> int:
     return code
 
 
-def _rows_any(t: torch.Tensor, what: str) -> torch.Tensor:
-    """[..., c] of any of the three types -> a 2-d view whose rows are contiguous (row stride >= c), or a copy."""
+def _rows_any(t: torch.Tensor, what: str):
+    """[..., c] of any of the three types -> (a tensor whose rows are contiguous: t itself, a 2-d view or a copy; number of rows; row
+    stride)."""
     _elem(t, what)
     if t.dim() < 1 or t.shape[-1] < 1:
         raise ValueError(f"{what}: expected at least one value in the last dimension, got shape {tuple(t.shape)}")
-    t2 = t.reshape(-1, t.shape[-1])
-    if t2.stride(1) != 1 or (t2.shape[0] > 1 and t2.stride(0) < t2.shape[1]):
+    c = t.shape[-1]
+    if t.is_contiguous():
+        return t, t.numel() // c, c
+    t2 = t.reshape(-1, c)
+    if t2.stride(1) != 1 or (t2.shape[0] > 1 and t2.stride(0) < c):
         t2 = t2.contiguous()
-    return t2
+    return t2, t2.shape[0], _ld(t2)
 
 
 def _vector(t: Optional[torch.Tensor], size: int, like: torch.Tensor, what: str) -> Optional[torch.Tensor]:
     """A bias or a norm's weight: [size], in `like`'s type or fp32, on its device."""
     if t is None:
         return None
-    if tuple(t.shape) != (size,):
+    if t.dim() != 1 or t.shape[0] != size:
         raise ValueError(f"{what}: expected shape ({size},), got {tuple(t.shape)}")
     if t.device != like.device or t.dtype not in (like.dtype, torch.float32):
         raise TypeError(f"{what}: expected {like.dtype} or fp32 on {like.device}, got {t.dtype} on {t.device}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 # A launch on the tensors' device and its current stream, bracketed with events when PROFILE is a list.  (Torch's device context and
@@ -966,42 +970,49 @@ def _differentiable_once(backward):
     return run
 
 
+# (In the backward passes below every tensor operation counts double: they run on autograd's own thread, whose core finds none of
+# the interpreter's objects in its caches.  What can be known beforehand is left in the context by the forward pass.)
+def _layer_norm_forward(x: torch.Tensor, w, b, eps: float, need_grad: bool):
+    """-> (y, what the backward pass needs: None, or the tensors to save and the arguments that are no tensors)"""
+    x2, n, ld = _rows_any(x, "x")
+    c, dev, dtype = x.shape[-1], x2.device, x2.dtype
+    wc, bc = _vector(w, c, x2, "weight"), _vector(b, c, x2, "bias")
+    w_dtype = dtype if wc is None and bc is None else (bc if wc is None else wc).dtype
+    if wc is not None and bc is not None and bc.dtype != w_dtype:
+        raise TypeError(f"layer_norm: weight is {wc.dtype}, bias {bc.dtype}")
+    y = torch.empty(x.shape, dtype=dtype, device=dev)
+    stats = torch.empty((3, n), dtype=torch.float32, device=dev) if need_grad else None
+    kind, w_kind = ELEM_TYPES[dtype], ELEM_TYPES[w_dtype]
+    _launch(dev, "layer_norm", 2 * n * c * dtype.itemsize, lib.nerf_layer_norm_fwd, n, c, kind, x2.data_ptr(), ld, w_kind, _ptr(wc), _ptr(bc), eps,
+            y.data_ptr(), c, _ptr(stats))
+    if not need_grad:
+        return y, None
+    return y, ((x2, wc, stats), (n, c, ld, kind, w_kind, dtype, w_dtype, dev, lib.nerf_layer_norm_workspace_floats(n, c)))
+
+
 class _LayerNorm(torch.autograd.Function):
     """Layer norm over the last dimension, forward and backward in libnerf_hip.so (layer_norm.hip)."""
 
     @staticmethod
-    def forward(ctx, x, w, b, eps, need_grad):
-        x2 = _rows_any(x, "x")
-        n, c = x2.shape
-        dev, dtype = x2.device, x2.dtype
-        wc, bc = _vector(w, c, x2, "weight"), _vector(b, c, x2, "bias")
-        w_dtype = dtype if wc is None and bc is None else (bc if wc is None else wc).dtype
-        if wc is not None and bc is not None and bc.dtype != w_dtype:
-            raise TypeError(f"layer_norm: weight is {wc.dtype}, bias {bc.dtype}")
-        y = torch.empty(x.shape, dtype=dtype, device=dev)
-        stats = torch.empty((3, n), dtype=torch.float32, device=dev) if need_grad else None
-        _launch(dev, "layer_norm", 2 * n * c * x2.element_size(), lib.nerf_layer_norm_fwd, n, c, ELEM_TYPES[dtype], x2.data_ptr(), _ld(x2),
-                ELEM_TYPES[w_dtype], _ptr(wc), _ptr(bc), eps, y.data_ptr(), c, _ptr(stats))
-        if need_grad:
-            ctx.save_for_backward(x2, wc, stats)
-            ctx.w_dtype = w_dtype
+    def forward(ctx, x, w, b, eps):
+        y, (saved, ctx.args) = _layer_norm_forward(x, w, b, eps, True)
+        ctx.save_for_backward(*saved)
         return y
 
     @staticmethod
     @_differentiable_once
     def backward(ctx, dy):
         x2, wc, stats = ctx.saved_tensors
-        n, c = x2.shape
-        dev, dtype, w_dtype = x2.device, x2.dtype, ctx.w_dtype
-        dy2 = _rows_any(dy, "grad")
-        need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
+        n, c, ld, kind, w_kind, dtype, w_dtype, dev, floats = ctx.args
+        dy2, _, ld_dy = _rows_any(dy, "grad")
+        need_dx, need_dw, need_db, _ = ctx.needs_input_grad
         dx = torch.empty(dy.shape, dtype=dtype, device=dev) if need_dx else None
         dw = torch.empty((c,), dtype=w_dtype, device=dev) if need_dw else None
         db = torch.empty((c,), dtype=w_dtype, device=dev) if need_db else None
-        ws = torch.empty((lib.nerf_layer_norm_workspace_floats(n, c),), dtype=torch.float32, device=dev) if need_dw or need_db else None
-        _launch(dev, "layer_norm_bwd", 3 * n * c * x2.element_size(), lib.nerf_layer_norm_bwd, n, c, ELEM_TYPES[dtype], x2.data_ptr(), _ld(x2),
-                dy2.data_ptr(), _ld(dy2), ELEM_TYPES[w_dtype], _ptr(wc), stats.data_ptr(), _ptr(dx), c, _ptr(dw), _ptr(db), _ptr(ws))
-        return dx, dw, db, None, None
+        ws = torch.empty((floats,), dtype=torch.float32, device=dev) if need_dw or need_db else None
+        _launch(dev, "layer_norm_bwd", 3 * n * c * dtype.itemsize, lib.nerf_layer_norm_bwd, n, c, kind, x2.data_ptr(), ld, dy2.data_ptr(), ld_dy,
+                w_kind, _ptr(wc), stats.data_ptr(), _ptr(dx), c, _ptr(dw), _ptr(db), _ptr(ws))
+        return dx, dw, db, None
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -1011,8 +1022,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     gradients are summed in a fixed order (bitwise reproducible)."""
     if not eps >= 0.0:
         raise ValueError(f"layer_norm: eps={eps}")
-    need = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias))
-    return _LayerNorm.apply(x, weight, bias, float(eps), need)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+        return _LayerNorm.apply(x, weight, bias, float(eps))
+    return _layer_norm_forward(x, weight, bias, float(eps), False)[0]
 
 
 class Fp8Rows:
@@ -1041,14 +1053,14 @@ class Fp8Rows:
 
 
 def _fp8_empty(rows: int, k: int, dev):
-    return (torch.empty((rows, int(lib.nerf_fp8_code_stride(k))), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn),
+    return (torch.empty((rows, int(lib.nerf_fp8_code_stride(k))), dtype=torch.float8_e4m3fn, device=dev),
             torch.empty((rows, int(lib.nerf_fp8_scale_stride(k))), dtype=torch.uint8, device=dev))
 
 
-def _quantize(x2: torch.Tensor, want: bool, want_t: bool, mask: Optional[torch.Tensor] = None, sum_dtype=None):
-    """x2 [rows, cols] -> (Fp8Rows of x2, Fp8Rows of its transpose, column sums), each None unless asked for; one pass over x2."""
-    rows, cols = x2.shape
-    dev = x2.device
+def _quantize(x: torch.Tensor, want: bool, want_t: bool, mask: Optional[torch.Tensor] = None, sum_dtype=None):
+    """A matrix [rows, cols] -> (Fp8Rows of it, Fp8Rows of its transpose, column sums), each None unless asked for; one pass over it."""
+    x2, rows, ld = _rows_any(x, "x")
+    cols, dev = x.shape[-1], x2.device
     q, qt, sums, ws = (None, None), (None, None), None, None
     if want:
         q = _fp8_empty(rows, cols, dev)
@@ -1058,7 +1070,7 @@ def _quantize(x2: torch.Tensor, want: bool, want_t: bool, mask: Optional[torch.T
         sums = torch.empty((cols,), dtype=sum_dtype, device=dev)
         ws = torch.empty(lib.nerf_fp8_quantize_workspace_floats(rows, cols), dtype=torch.float32, device=dev)
     _launch(dev, "fp8_quantize", rows * cols * (x2.element_size() + int(want) + int(want_t)), lib.nerf_fp8_quantize, rows, cols,
-            ELEM_TYPES[x2.dtype], x2.data_ptr(), _ld(x2), _ptr(mask), 0 if mask is None else _ld(mask), _ptr(q[0]), _ptr(q[1]), _ptr(qt[0]),
+            ELEM_TYPES[x2.dtype], x2.data_ptr(), ld, _ptr(mask), 0 if mask is None else _ld(mask), _ptr(q[0]), _ptr(q[1]), _ptr(qt[0]),
             _ptr(qt[1]), 0 if sums is None else ELEM_TYPES[sum_dtype], _ptr(sums), _ptr(ws))
     return Fp8Rows(*q, cols) if want else None, Fp8Rows(*qt, rows) if want_t else None, sums
 
@@ -1069,7 +1081,7 @@ def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
     becomes NaN."""
     if x.dim() != 2:
         raise ValueError(f"quantize_fp8: expected a matrix, got shape {tuple(x.shape)}")
-    return _quantize(_rows_any(x.detach(), "x"), True, False)[0]
+    return _quantize(x.detach(), True, False)[0]
 
 
 def matmul_fp8(a: Fp8Rows, b: Fp8Rows, bias: Optional[torch.Tensor] = None, relu: bool = False,
@@ -1099,21 +1111,22 @@ def _bytes(count: int, dev) -> Optional[torch.Tensor]:
     return torch.empty((count,), dtype=torch.uint8, device=dev) if count else None
 
 
-def _linear_fp8_forward(x: torch.Tensor, x2: torch.Tensor, w2, n_out: int, b, relu: bool, need_dx: bool, need_dw: bool):
-    """-> (y, what the backward pass needs of x and w in 8 bits); w2: a matrix of rows, or an Fp8Rows."""
-    n, n_in = x2.shape
-    dev, kind = x2.device, ELEM_TYPES[x2.dtype]
+def _linear_fp8_forward(x: torch.Tensor, weight, b, relu: bool, need_dx: bool, need_dw: bool):
+    """weight: a matrix, or an Fp8Rows -> (y, what the backward pass needs of x and the weight in 8 bits, the sizes)"""
+    x2, n, ld = _rows_any(x, "x")
+    n_in, dev, kind = x.shape[-1], x2.device, ELEM_TYPES[x2.dtype]
+    if isinstance(weight, Fp8Rows):
+        n_out, w_args = weight.rows, (0, None, 0, weight.codes.data_ptr(), weight.scales.data_ptr())
+    else:
+        w2, n_out, ldw = _rows_any(weight, "weight")
+        w_args = (ELEM_TYPES[w2.dtype], w2.data_ptr(), ldw, None, None)
     bias = _vector(b, n_out, x2, "bias")
     y = torch.empty(x.shape[:-1] + (n_out,), dtype=x2.dtype, device=dev)
     kept = _bytes(lib.nerf_linear_fp8_kept_bytes(n, n_in, n_out, need_dx, need_dw), dev) if need_dx or need_dw else None
     ws = _bytes(lib.nerf_linear_fp8_workspace_bytes(n, n_in, n_out, kind, 0, 0), dev)
-    if isinstance(w2, Fp8Rows):
-        weight = (0, None, 0, w2.codes.data_ptr(), w2.scales.data_ptr())
-    else:
-        weight = (ELEM_TYPES[w2.dtype], w2.data_ptr(), _ld(w2), None, None)
-    _launch(dev, "linear_fp8", 2 * n * n_in * n_out, lib.nerf_linear_fp8_fwd, n, n_in, n_out, kind, x2.data_ptr(), _ld(x2), *weight,
+    _launch(dev, "linear_fp8", 2 * n * n_in * n_out, lib.nerf_linear_fp8_fwd, n, n_in, n_out, kind, x2.data_ptr(), ld, *w_args,
             kind if bias is None else ELEM_TYPES[bias.dtype], _ptr(bias), int(relu), y.data_ptr(), _ptr(kept), need_dx, need_dw, _ptr(ws))
-    return y, kept
+    return y, kept, (n, n_in, n_out, kind, dev)
 
 
 class _LinearFp8(torch.autograd.Function):
@@ -1121,36 +1134,34 @@ class _LinearFp8(torch.autograd.Function):
     unquantised values; what the backward pass needs of x and w is kept in 8 bits."""
 
     @staticmethod
-    def forward(ctx, x, w, b, relu, need_grad):
-        x2, w2 = _rows_any(x, "x"), _rows_any(w, "weight")
-        need_dx, need_dw = need_grad and ctx.needs_input_grad[0], need_grad and ctx.needs_input_grad[1]
-        n_out, n_in = w2.shape
-        y, kept = _linear_fp8_forward(x, x2, w2, n_out, b, relu, need_dx, need_dw)
-        if need_grad:
-            ctx.save_for_backward(kept, y if relu else None)
-            ctx.args = (x2.shape[0], n_in, n_out, need_dx, need_dw, w.dtype, None if b is None else b.dtype)
+    def forward(ctx, x, w, b, relu):
+        need_dx, need_dw = ctx.needs_input_grad[:2]
+        y, kept, sizes = _linear_fp8_forward(x, w, b, relu, need_dx, need_dw)
+        ctx.save_for_backward(kept, y if relu else None)
+        n, n_in, n_out, kind, _ = sizes
+        w_kind = ELEM_TYPES[w.dtype]
+        ctx.args = sizes + (need_dx, need_dw, x.dtype, w.dtype, w_kind, None if b is None else b.dtype,
+                            lib.nerf_linear_fp8_workspace_bytes(n, n_in, n_out, kind, w_kind, 1))
         return y
 
     @staticmethod
     @_differentiable_once
     def backward(ctx, dy):
         kept, y = ctx.saved_tensors
-        n, n_in, n_out, kept_dx, kept_dw, w_dtype, b_dtype = ctx.args
-        need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
-        dy2 = _rows_any(dy, "grad")
-        dev, kind = dy2.device, ELEM_TYPES[dy2.dtype]
-        dx = torch.empty(dy.shape[:-1] + (n_in,), dtype=dy2.dtype, device=dev) if need_dx else None
+        n, n_in, n_out, kind, dev, kept_dx, kept_dw, dtype, w_dtype, w_kind, b_dtype, count = ctx.args
+        need_dx, need_dw, need_db, _ = ctx.needs_input_grad
+        dx = torch.empty(dy.shape[:-1] + (n_in,), dtype=dtype, device=dev) if need_dx else None
         if n == 0:
             dw = torch.zeros((n_out, n_in), dtype=w_dtype, device=dev) if need_dw else None
             db = torch.zeros((n_out,), dtype=b_dtype, device=dev) if need_db else None
-            return dx, dw, db, None, None
+            return dx, dw, db, None
+        dy2, _, ld = _rows_any(dy, "grad")
         dw = torch.empty((n_out, n_in), dtype=w_dtype, device=dev) if need_dw else None
         db = torch.empty((n_out,), dtype=b_dtype, device=dev) if need_db else None
-        ws = _bytes(lib.nerf_linear_fp8_workspace_bytes(n, n_in, n_out, kind, ELEM_TYPES[w_dtype], 1), dev)
-        _launch(dev, "linear_fp8_bwd", 4 * n * n_in * n_out, lib.nerf_linear_fp8_bwd, n, n_in, n_out, kind, dy2.data_ptr(), _ld(dy2), _ptr(y),
-                _ptr(kept), kept_dx, kept_dw, _ptr(dx), ELEM_TYPES[w_dtype], _ptr(dw), 0 if db is None else ELEM_TYPES[b_dtype], _ptr(db),
-                ws.data_ptr())
-        return dx, dw, db, None, None
+        ws = torch.empty((count,), dtype=torch.uint8, device=dev)
+        _launch(dev, "linear_fp8_bwd", 4 * n * n_in * n_out, lib.nerf_linear_fp8_bwd, n, n_in, n_out, kind, dy2.data_ptr(), ld, _ptr(y), _ptr(kept),
+                kept_dx, kept_dw, _ptr(dx), w_kind, _ptr(dw), 0 if db is None else ELEM_TYPES[b_dtype], _ptr(db), ws.data_ptr())
+        return dx, dw, db, None
 
 
 def linear_fp8(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = None, relu: bool = False) -> torch.Tensor:
@@ -1161,16 +1172,16 @@ def linear_fp8(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = None, rel
     if isinstance(weight, Fp8Rows):
         if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
             raise ValueError("linear_fp8: a weight held in 8 bits has no backward pass; call it under torch.no_grad()")
-        x2 = _rows_any(x, "x")
-        if x2.shape[1] != weight.k:
-            raise ValueError(f"linear_fp8: x has {x2.shape[1]} values per row, the weight k={weight.k}")
-        if weight.codes.device != x2.device:
-            raise TypeError(f"linear_fp8: x on {x2.device}, the weight on {weight.codes.device}")
-        return _linear_fp8_forward(x, x2, weight, weight.rows, bias, bool(relu), False, False)[0]
+        if x.dim() < 1 or x.shape[-1] != weight.k:
+            raise ValueError(f"linear_fp8: x {tuple(x.shape)} against a weight with k={weight.k}")
+        if weight.codes.device != x.device:
+            raise TypeError(f"linear_fp8: x on {x.device}, the weight on {weight.codes.device}")
+        return _linear_fp8_forward(x, weight, bias, bool(relu), False, False)[0]
     _elem(x, "x")
     if weight.dim() != 2 or x.dim() < 1 or weight.shape[1] != x.shape[-1]:
         raise ValueError(f"linear_fp8: x {tuple(x.shape)} against weight {tuple(weight.shape)}")
     if weight.device != x.device or weight.dtype not in (x.dtype, torch.float32):
         raise TypeError(f"linear_fp8: expected a weight in {x.dtype} or fp32 on {x.device}, got {weight.dtype} on {weight.device}")
-    need = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias))
-    return _LinearFp8.apply(x, weight, bias, bool(relu), need)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return _LinearFp8.apply(x, weight, bias, bool(relu))
+    return _linear_fp8_forward(x, weight, bias, bool(relu), False, False)[0]

@@ -20,6 +20,7 @@ namespace {
 
 constexpr int KB = 128;       // values of k that share a scale
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -272,11 +273,11 @@ __device__ __forceinline__ float finish(float v, const Product& p, int64_t col) 
     return v;
 }
 
+// a lane's 32 of the 128 bytes of a block: the 16 at 16 g and the 16 at 64 + 16 g (any division of k will do that both operands share;
+// with this one an instruction reads 64 bytes of a row together)
 __device__ __forceinline__ i32x8 load32(const uint8_t* p) {
-    const uint4 x = *reinterpret_cast<const uint4*>(p), y = *reinterpret_cast<const uint4*>(p + 16);
-    i32x8 r;
-    r[0] = x.x; r[1] = x.y; r[2] = x.z; r[3] = x.w; r[4] = y.x; r[5] = y.y; r[6] = y.z; r[7] = y.w;
-    return r;
+    const i32x4 x = *reinterpret_cast<const i32x4*>(p), y = *reinterpret_cast<const i32x4*>(p + 64);
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 // acc += a b^T over one block of k: a lane holds 32 of the 128 values of row (lane & 15) of either operand, and that row's scale byte
@@ -296,9 +297,10 @@ __device__ __forceinline__ f32x4 mul_decoded(i32x8 a, int sa, i32x8 b, int sb, f
     return acc;
 }
 
-// Few rows: a workgroup owns 16 columns of C and up to 16 MT rows; its waves take the blocks of k in turn, straight from memory into the
-// instruction's registers, and add up through LDS.
-constexpr int FEW_WAVES = 8;
+// Few rows: a workgroup owns 16 columns of C and up to 16 MT rows; each of its waves takes an eighth of the blocks of k, straight from
+// memory into the instruction's registers, four blocks requested at a time, and the waves add up through LDS.  The weight's codes
+// are read once: that is what bounds it.
+constexpr int FEW_WAVES = 8, FEW_U = 4;
 template <typename T, int MT>
 __global__ void __launch_bounds__(64 * FEW_WAVES) k_product_few(Product p) {
     constexpr bool F32 = sizeof(T) == 4;
@@ -306,25 +308,38 @@ __global__ void __launch_bounds__(64 * FEW_WAVES) k_product_few(Product p) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
     const int64_t j0 = (int64_t)blockIdx.x * 16, i0 = (int64_t)blockIdx.y * 16 * MT;
     const int64_t jb = j0 + r < p.n ? j0 + r : p.n - 1;
-    const uint8_t *bp = p.b + jb * p.ldk + 32 * g, *sbp = p.sb + jb * p.lds;
+    const uint8_t *bp = p.b + jb * p.ldk + 16 * g, *sbp = p.sb + jb * p.lds;
     const uint8_t *ap[MT], *sap[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int64_t ia = i0 + 16 * t + r < p.m ? i0 + 16 * t + r : p.m - 1;
-        ap[t] = p.a + ia * p.ldk + 32 * g;
+        ap[t] = p.a + ia * p.ldk + 16 * g;
         sap[t] = p.sa + ia * p.lds;
     }
     f32x4 acc[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[t] = f32x4{0, 0, 0, 0};
-    for (int kb = wave; kb < p.blocks; kb += FEW_WAVES) {
-        const i32x8 b = load32(bp + (int64_t)kb * KB);
-        const int sb = sbp[kb];
+    // (a wave's blocks in fours, whose scales are one word of a row)
+    const int fours = (p.blocks + 3) / 4, per = (fours + FEW_WAVES - 1) / FEW_WAVES;
+    const int q1 = (wave + 1) * per < fours ? (wave + 1) * per : fours;
+    for (int q = wave * per; q < q1; ++q) {
+        const int kb = 4 * q;
+        i32x8 b[FEW_U];
+#pragma unroll
+        for (int u = 0; u < FEW_U; ++u) b[u] = load32(bp + (int64_t)(kb + u < p.blocks ? kb + u : p.blocks - 1) * KB);
+        const unsigned sb = *reinterpret_cast<const unsigned*>(sbp + kb);
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            const i32x8 a = load32(ap[t] + (int64_t)kb * KB);
-            const int sa = sap[t][kb];
-            acc[t] = F32 ? mul_decoded(a, sa, b, sb, acc[t]) : mul_fp8(a, sa, b, sb, acc[t]);
+            const unsigned sa = *reinterpret_cast<const unsigned*>(sap[t] + kb);
+            i32x8 a[FEW_U];
+#pragma unroll
+            for (int u = 0; u < FEW_U; ++u) a[u] = load32(ap[t] + (int64_t)(kb + u < p.blocks ? kb + u : p.blocks - 1) * KB);
+#pragma unroll
+            for (int u = 0; u < FEW_U; ++u) {
+                if (kb + u >= p.blocks) break;
+                const int ea = (int)(sa >> 8 * u & 255u), eb = (int)(sb >> 8 * u & 255u);
+                acc[t] = F32 ? mul_decoded(a[u], ea, b[u], eb, acc[t]) : mul_fp8(a[u], ea, b[u], eb, acc[t]);
+            }
         }
     }
 #pragma unroll
@@ -380,7 +395,6 @@ struct Stage {      // one operand's rows on their way into LDS
     }
 };
 
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 // where a lane's 32 of the 64 bytes of either half of row `row` lie in an image: pieces 4 h + 2 g and the one behind it
 struct Piece {
     int x[2], y[2];
@@ -664,10 +678,12 @@ template <typename T>
 int product(const Product& p, int64_t k, int type, float* ws, hipStream_t stream) {
     const Plan plan = plan_of(p.m, p.n, k, type);
     if (plan.tile == 0) {
-        constexpr int MT = 4;
-        const int64_t gx = (p.n + 15) / 16, gy = (p.m + 16 * MT - 1) / (16 * MT);
+        const int mt = p.m <= 16 ? 1 : p.m <= 32 ? 2 : 4;
+        const int64_t gx = (p.n + 15) / 16, gy = (p.m + 16 * mt - 1) / (16 * mt);
         if (gx > 0x7fffff || gy > 65535) return fail(NERF_E_ARG, "nerf_fp8_matmul: %lld x %lld is more than one launch covers", (long long)p.m, (long long)p.n);
-        hipLaunchKernelGGL((k_product_few<T, MT>), dim3((unsigned)gx, (unsigned)gy), dim3(64 * FEW_WAVES), 0, stream, p);
+#define GO(MT) hipLaunchKernelGGL((k_product_few<T, MT>), dim3((unsigned)gx, (unsigned)gy), dim3(64 * FEW_WAVES), 0, stream, p)
+        if (mt == 1) GO(1); else if (mt == 2) GO(2); else GO(4);
+#undef GO
         return launched("nerf_fp8_matmul");
     }
     const int64_t tm = (p.m + plan.tile - 1) / plan.tile, tn = (p.n + plan.tile - 1) / plan.tile;

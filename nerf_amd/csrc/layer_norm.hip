@@ -15,16 +15,7 @@ namespace {
 constexpr int LN_THREADS = 256;
 constexpr int LN_SLICES = 1024;         // the most slices of the rows in the weight gradients' sums
 constexpr int64_t LN_HELD = 16384;      // rows up to this length are held in registers
-
-// a norm's weight or bias: fp32 or the rows' type, or absent
-template <typename T>
-struct Param {
-    const void* p;
-    int f32;
-    __device__ __forceinline__ float at(int64_t i, float absent) const {
-        return !p ? absent : f32 ? ((const float*)p)[i] : (float)((const T*)p)[i];
-    }
-};
+constexpr int LN_GROUPS = 2048;         // the most workgroups of the forward pass
 
 // VEC elements from any element's address (the memory system takes vector accesses at any alignment)
 template <typename T, int VEC>
@@ -56,6 +47,27 @@ __device__ __forceinline__ void write_row(T* row, int i, int c, const float (&in
             if (i + e < c) row[i + e] = (T)in[e];
     }
 }
+
+// a norm's weight or bias: fp32 or the rows' type, or absent
+template <typename T>
+struct Param {
+    const void* p;
+    int f32;
+    __device__ __forceinline__ float at(int64_t i, float absent) const {
+        return !p ? absent : f32 ? ((const float*)p)[i] : (float)((const T*)p)[i];
+    }
+    template <int VEC>
+    __device__ __forceinline__ void read(int i, int c, float absent, float (&out)[VEC]) const {      // zeros behind c
+        if (!p) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) out[e] = i + e < c ? absent : 0.0f;
+        } else if (f32) {
+            read_row<float, VEC>((const float*)p, i, c, out);
+        } else {
+            read_row<T, VEC>((const T*)p, i, c, out);
+        }
+    }
+};
 
 template <int CTRL>
 __device__ __forceinline__ float add_ror(float v) {
@@ -103,24 +115,39 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float* part) {
     }
 }
 
-// One pass over memory: a row is read once, held in registers for both passes of the statistics, and written once.
+// One pass over memory: a row is read once, held in registers for both passes of the statistics, and written once.  A workgroup stays
+// for many rows: the weight and the bias are read once, and the next row is under way while this one is worked on.
 template <typename T, typename S>
 __global__ void __launch_bounds__(S::THREADS) k_ln_fwd_held(int64_t n, int c, const T* __restrict__ x, int64_t ldx, Param<T> w, Param<T> b, float eps,
                                                             T* __restrict__ y, int64_t ldy, float* __restrict__ stats) {
     __shared__ float part[2][2 * S::WPR];
     const int lane = threadIdx.x % S::PER_ROW, slot = threadIdx.x / S::PER_ROW;
     const float fc = (float)c;
+    Loose<T, S::VEC> next[S::CH];
+    auto request = [&](int64_t row) {
+        const T* xr = x + (row < n ? row : n - 1) * ldx;
+#pragma unroll
+        for (int k = 0; k < S::CH; ++k) next[k] = read_raw<T, S::VEC>(xr, (k * S::PER_ROW + lane) * S::VEC, c);
+    };
+    request((int64_t)blockIdx.x * S::ROWS + slot);
+    float wv[S::CH][S::VEC], bv[S::CH][S::VEC];
+#pragma unroll
+    for (int k = 0; k < S::CH; ++k) {
+        const int i = (k * S::PER_ROW + lane) * S::VEC;
+        w.read(i, c, 1.0f, wv[k]);
+        b.read(i, c, 0.0f, bv[k]);
+    }
     for (int64_t row0 = (int64_t)blockIdx.x * S::ROWS; row0 < n; row0 += (int64_t)gridDim.x * S::ROWS) {
         const int64_t row = row0 + slot;
-        const bool live = row < n;
-        const T* xr = x + (live ? row : n - 1) * ldx;
         float v[S::CH][S::VEC], s[1] = {0.0f};
-#pragma unroll
-        for (int k = 0; k < S::CH; ++k) read_row<T, S::VEC>(xr, (k * S::PER_ROW + lane) * S::VEC, c, v[k]);
 #pragma unroll
         for (int k = 0; k < S::CH; ++k)
 #pragma unroll
-            for (int e = 0; e < S::VEC; ++e) s[0] += v[k][e];
+            for (int e = 0; e < S::VEC; ++e) {
+                v[k][e] = (float)next[k].e[e];
+                s[0] += v[k][e];
+            }
+        if (row0 + (int64_t)gridDim.x * S::ROWS < n) request(row + (int64_t)gridDim.x * S::ROWS);
         row_sum<S, 1>(s, part[0]);
         const float mu1 = s[0] / fc;
         float d[2] = {0.0f, 0.0f};
@@ -137,25 +164,19 @@ __global__ void __launch_bounds__(S::THREADS) k_ln_fwd_held(int64_t n, int c, co
         row_sum<S, 2>(d, part[1]);
         const float mu2 = d[0] / fc, var = fmaxf(d[1] / fc - mu2 * mu2, 0.0f);
         const float r = (d[1] != d[1]) ? d[1] : 1.0f / sqrtf(var + eps);      // (fmaxf drops a NaN)
-        if (live) {
+        if (row >= n) continue;
 #pragma unroll
-            for (int k = 0; k < S::CH; ++k) {
-                const int i = (k * S::PER_ROW + lane) * S::VEC;
-                if (i >= c) continue;
-                float o[S::VEC], wv[S::VEC], bv[S::VEC];
+        for (int k = 0; k < S::CH; ++k) {
+            const int i = (k * S::PER_ROW + lane) * S::VEC;
+            if (i >= c) continue;
 #pragma unroll
-                for (int e = 0; e < S::VEC; ++e) { wv[e] = 1.0f; bv[e] = 0.0f; }
-                if (w.p) { if (w.f32) read_row<float, S::VEC>((const float*)w.p, i, c, wv); else read_row<T, S::VEC>((const T*)w.p, i, c, wv); }
-                if (b.p) { if (b.f32) read_row<float, S::VEC>((const float*)b.p, i, c, bv); else read_row<T, S::VEC>((const T*)b.p, i, c, bv); }
-#pragma unroll
-                for (int e = 0; e < S::VEC; ++e) o[e] = (v[k][e] - mu2) * r * wv[e] + bv[e];
-                write_row<T, S::VEC>(y + row * ldy, i, c, o);
-            }
-            if (stats && lane == 0) {
-                stats[row] = mu1;
-                stats[n + row] = mu2;
-                stats[2 * n + row] = r;
-            }
+            for (int e = 0; e < S::VEC; ++e) v[k][e] = (v[k][e] - mu2) * r * wv[k][e] + bv[k][e];
+            write_row<T, S::VEC>(y + row * ldy, i, c, v[k]);
+        }
+        if (stats && lane == 0) {
+            stats[row] = mu1;
+            stats[n + row] = mu2;
+            stats[2 * n + row] = r;
         }
     }
 }
@@ -163,7 +184,7 @@ __global__ void __launch_bounds__(S::THREADS) k_ln_fwd_held(int64_t n, int c, co
 // x and dy are read once: dx is written and the weight's and bias's sums of this workgroup's rows stay in registers; they are left as
 // partial[workgroup][0 | 1][column].
 template <typename T, typename S>
-__global__ void __launch_bounds__(S::THREADS) k_ln_bwd_held(int64_t n, int c, const T* __restrict__ x, int64_t ldx, const T* __restrict__ dy,
+__global__ void __launch_bounds__(S::THREADS, S::WPR > 4 ? 4 : 1) k_ln_bwd_held(int64_t n, int c, const T* __restrict__ x, int64_t ldx, const T* __restrict__ dy,
                                                             int64_t lddy, Param<T> w, const float* __restrict__ stats, T* __restrict__ dx,
                                                             int64_t lddx, float* __restrict__ partial) {
     __shared__ float part[2][2 * S::WPR];
@@ -172,14 +193,12 @@ __global__ void __launch_bounds__(S::THREADS) k_ln_bwd_held(int64_t n, int c, co
     float wv[S::CH][S::VEC], sw[S::CH][S::VEC], sb[S::CH][S::VEC];
 #pragma unroll
     for (int k = 0; k < S::CH; ++k) {
-        const int i = (k * S::PER_ROW + lane) * S::VEC;
+        w.read((k * S::PER_ROW + lane) * S::VEC, c, 1.0f, wv[k]);
 #pragma unroll
-        for (int e = 0; e < S::VEC; ++e) {
-            wv[k][e] = i + e < c ? w.at(i + e, 1.0f) : 0.0f;
-            sw[k][e] = sb[k][e] = 0.0f;
-        }
+        for (int e = 0; e < S::VEC; ++e) sw[k][e] = sb[k][e] = 0.0f;
     }
-    // (the next row is under way while this one is worked on)
+    // (the next row is under way while this one is worked on, where a thread's registers allow it)
+    constexpr bool AHEAD = S::WPR <= 4;
     Loose<T, S::VEC> nx[S::CH], ng[S::CH];
     auto request = [&](int64_t row) {
         const int64_t at = row < n ? row : n - 1;
@@ -190,12 +209,13 @@ __global__ void __launch_bounds__(S::THREADS) k_ln_bwd_held(int64_t n, int c, co
             ng[k] = read_raw<T, S::VEC>(dy + at * lddy, i, c);
         }
     };
-    request((int64_t)blockIdx.x * S::ROWS + slot);
+    if (AHEAD) request((int64_t)blockIdx.x * S::ROWS + slot);
     int odd = 0;
     for (int64_t row0 = (int64_t)blockIdx.x * S::ROWS; row0 < n; row0 += (int64_t)gridDim.x * S::ROWS, odd ^= 1) {
         const int64_t row = row0 + slot;
         const bool live = row < n;
         const int64_t at = live ? row : n - 1;
+        if (!AHEAD) request(row);
         const float mu1 = stats[at], mu2 = stats[n + at], r = stats[2 * n + at];
         float xh[S::CH][S::VEC], g[S::CH][S::VEC], s[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -205,7 +225,7 @@ __global__ void __launch_bounds__(S::THREADS) k_ln_bwd_held(int64_t n, int c, co
                 xh[k][e] = (float)nx[k].e[e];
                 g[k][e] = (float)ng[k].e[e];
             }
-        if (row0 + (int64_t)gridDim.x * S::ROWS < n) request(row + (int64_t)gridDim.x * S::ROWS);
+        if (AHEAD && row0 + (int64_t)gridDim.x * S::ROWS < n) request(row + (int64_t)gridDim.x * S::ROWS);
 #pragma unroll
         for (int k = 0; k < S::CH; ++k) {
             const int i = (k * S::PER_ROW + lane) * S::VEC;
@@ -352,17 +372,17 @@ __global__ void __launch_bounds__(LN_THREADS) k_ln_dw(int64_t n, int c, const T*
     partial[((int64_t)blockIdx.y * 2 + 1) * c + col] = sb;
 }
 
-// the slices' sums of 64 columns (of dw's C, then db's), in fp64, sixteen slices at a time
-constexpr int LF_ROWS = 16;
+// the slices' sums of 32 columns (of dw's C, then db's), in fp64, 32 slices at a time
+constexpr int LF_COLS = 32, LF_ROWS = 32;
 template <typename W>
-__global__ void __launch_bounds__(64 * LF_ROWS) k_ln_finish(int slices, int c, const float* __restrict__ partial, W* __restrict__ dw,
-                                                            W* __restrict__ db) {
-    __shared__ double red[LF_ROWS][64];
-    const int lane = threadIdx.x & 63, row = threadIdx.x >> 6;
-    const int64_t col = (int64_t)blockIdx.x * 64 + lane;
+__global__ void __launch_bounds__(LF_COLS * LF_ROWS) k_ln_finish(int slices, int c, const float* __restrict__ partial, W* __restrict__ dw,
+                                                                 W* __restrict__ db) {
+    __shared__ double red[LF_ROWS][LF_COLS + 1];
+    const int lane = threadIdx.x % LF_COLS, row = threadIdx.x / LF_COLS;
+    const int64_t col = (int64_t)blockIdx.x * LF_COLS + lane;
     double s = 0.0;
     if (col < 2 * (int64_t)c) {
-#pragma unroll 4
+#pragma unroll 8
         for (int z = row; z < slices; z += LF_ROWS) s += (double)partial[(int64_t)z * 2 * c + col];
     }
     red[row][lane] = s;
@@ -397,7 +417,7 @@ int with_shape(int64_t c, F&& f) {
 int slices_of(int64_t n, int64_t c) {
     if (n < 1) return 1;
     const int rows = c > LN_HELD ? 1 : with_shape(c, [](auto s) { return decltype(s)::ROWS; });
-    const int64_t groups = (n + rows - 1) / rows, most = c <= 2048 ? LN_SLICES : LN_SLICES / 2;
+    const int64_t groups = (n + rows - 1) / rows, most = c <= 2048 ? LN_SLICES : c <= 4096 ? LN_SLICES * 3 / 4 : LN_SLICES / 2;
     return (int)(groups < most ? groups : most);
 }
 
@@ -413,7 +433,7 @@ int fwd(int64_t n, int c, const void* x, int64_t ldx, int w_f32, const void* w, 
     return with_shape(c, [&](auto shape) {
         using S = decltype(shape);
         const int64_t groups = (n + S::ROWS - 1) / S::ROWS;
-        hipLaunchKernelGGL((k_ln_fwd_held<T, S>), dim3((unsigned)(groups < 8192 ? groups : 8192)), dim3(S::THREADS), 0, stream, n, c, (const T*)x,
+        hipLaunchKernelGGL((k_ln_fwd_held<T, S>), dim3((unsigned)(groups < LN_GROUPS ? groups : LN_GROUPS)), dim3(S::THREADS), 0, stream, n, c, (const T*)x,
                            ldx, wp, bp, eps, (T*)y, ldy, stats);
         return launched("nerf_layer_norm_fwd");
     });
@@ -449,9 +469,9 @@ int bwd(int64_t n, int c, const void* x, int64_t ldx, const void* dy, int64_t ld
         });
     }
     if (rc || !part) return rc;
-    const dim3 grid((unsigned)((2 * (int64_t)c + 63) / 64));
-    if (w_f32) hipLaunchKernelGGL((k_ln_finish<float>), grid, dim3(64 * LF_ROWS), 0, stream, slices, c, part, (float*)dw, (float*)db);
-    else hipLaunchKernelGGL((k_ln_finish<T>), grid, dim3(64 * LF_ROWS), 0, stream, slices, c, part, (T*)dw, (T*)db);
+    const dim3 grid((unsigned)((2 * (int64_t)c + LF_COLS - 1) / LF_COLS));
+    if (w_f32) hipLaunchKernelGGL((k_ln_finish<float>), grid, dim3(LF_COLS * LF_ROWS), 0, stream, slices, c, part, (float*)dw, (float*)db);
+    else hipLaunchKernelGGL((k_ln_finish<T>), grid, dim3(LF_COLS * LF_ROWS), 0, stream, slices, c, part, (T*)dw, (T*)db);
     return launched("nerf_layer_norm_bwd (sums)");
 }
 

@@ -213,6 +213,11 @@ def _address(values: array) -> int:
 
 
 _data_ptr, _numel, _is_contiguous, _get_device = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device
+_dtype, _layout, _grad = operator.attrgetter("dtype"), operator.attrgetter("layout"), operator.attrgetter("grad")
+
+
+def _all_are(values, one) -> bool:
+    return all(map(operator.is_, values, itertools.repeat(one)))
 
 
 class _Launch:
@@ -222,7 +227,7 @@ class _Launch:
     def __init__(self, device, dtype, index, params, states):
         self.device, self.dtype, self.kind = device, dtype, ELEM_TYPES[dtype]
         self.index, self.params = index, params
-        self.devices = array("q", [device.index] * len(index))
+        self.devices = array("q", [device.index] * len(params))
         self.counts = array("q", map(_numel, params))
         self.pointers = {"params": array("Q", map(_data_ptr, params))}
         self.bytes = 0
@@ -234,10 +239,10 @@ class _Launch:
 
     def take(self, all_grads):
         """This step's gradients: (addresses, the tensors they belong to)."""
-        grads = [all_grads[i] for i in self.index]
-        if not all(g.layout is torch.strided for g in grads):
+        grads = all_grads if self.index is None else [all_grads[i] for i in self.index]
+        if not _all_are(map(_layout, grads), torch.strided):
             raise TypeError("AdamW: sparse gradients are not supported")
-        if not all(g.dtype is self.dtype for g in grads) or array("q", map(_get_device, grads)) != self.devices:
+        if not _all_are(map(_dtype, grads), self.dtype) or array("q", map(_get_device, grads)) != self.devices:
             raise TypeError(f"AdamW: a gradient is not in {self.dtype} on {self.device}, as its parameter is")
         if array("q", map(_numel, grads)) != self.counts:
             raise ValueError("AdamW: a gradient has another size than its parameter")
@@ -253,7 +258,7 @@ class _Plan:
     __slots__ = ("params", "absent", "states", "held", "pointed", "addresses", "live", "counts", "launches")
 
     def __init__(self, opt, params, grads):
-        self.params, self.absent = list(params), [g is None for g in grads]
+        self.params, self.absent = list(params), list(map(operator.is_, grads, itertools.repeat(None)))
         lists = {}
         for i, (p, g) in enumerate(zip(params, grads)):
             if g is None:
@@ -272,11 +277,11 @@ class _Plan:
         self.pointed = self.live + [t for t in self.held if torch.is_tensor(t)]
         self.addresses = array("Q", map(_data_ptr, self.pointed))
         self.counts = array("q", map(_numel, self.live))
-        self.launches = [_Launch(device, dtype, index, [params[i] for i in index], [state_of[id(params[i])] for i in index])
-                         for (device, dtype), index in lists.items()]
+        self.launches = [_Launch(device, dtype, index if len(index) < len(self.params) else None, [params[i] for i in index],
+                                 [state_of[id(params[i])] for i in index]) for (device, dtype), index in lists.items()]
 
     def stands(self, params, grads) -> bool:
-        if len(params) != len(self.params) or not all(map(operator.is_, params, self.params)) or [g is None for g in grads] != self.absent:
+        if len(params) != len(self.params) or not all(map(operator.is_, params, self.params)) or list(map(operator.is_, grads, itertools.repeat(None))) != self.absent:
             return False
         held = list(itertools.chain.from_iterable(map(dict.values, self.states)))
         return (len(held) == len(self.held) and all(map(operator.is_, held, self.held))
@@ -362,8 +367,7 @@ class AdamW(torch.optim.Optimizer):
         return st
 
     # ---- the step ------------------------------------------------------------------------------------
-    @torch.no_grad()
-    def step(self, closure=None):
+    def step(self, closure=None):      # (nothing here is recorded by autograd: the library writes through addresses)
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -373,7 +377,7 @@ class AdamW(torch.optim.Optimizer):
         work = []
         for group in self.param_groups:      # (everything is checked before anything is launched)
             self._check_hyper(group["lr"], group["betas"], group["eps"], group["weight_decay"])
-            grads = [p.grad for p in group["params"]]
+            grads = list(map(_grad, group["params"]))
             plan = self._plans.get(id(group)) if known else None
             if plan is None or not plan.stands(group["params"], grads):
                 plan = self._plans[id(group)] = _Plan(self, group["params"], grads)

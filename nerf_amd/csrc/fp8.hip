@@ -364,8 +364,9 @@ __global__ void __launch_bounds__(64 * FEW_WAVES) k_product_few(Product p) {
 // halves of 64: while the first multiplies out of registers, the second's fragments are read, after which the image is done with:
 // behind the block's one barrier, while the second half multiplies, the rows of the block after the next are asked for in its place and
 // the first fragments of the next block are read.  So a request has one and a half blocks of multiplication to arrive and a
-// read half a block; neither is waited for.  The 16-byte pieces of a row are stored in the order piece ^ (row & 7), so that eight
-// neighbouring rows' reads of one piece cover all banks.
+// read half a block; neither is waited for.  The 16-byte pieces of a row are stored in the order piece ^ (row / 2 & 7): the sixteen
+// lanes whose 16-byte reads the LDS serves together hold rows that differ in this and the row's parity, so they cover all 64 banks
+// (piece ^ (row & 7) cost as many cycles again in conflicts).
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ f32x16 mul32_fp8(i32x8 a, int sa, i32x8 b, int sb, f32x16 acc) {
@@ -386,7 +387,7 @@ struct Stage {      // one operand's rows on their way into LDS
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int row = 8 * (wave + 4 * i) + r;
-            offset[i] = (unsigned)(row < last ? row : last) * (unsigned)ldk + (((lane & 7) ^ r) << 4);
+            offset[i] = (unsigned)(row < last ? row : last) * (unsigned)ldk + (((lane & 7) ^ (row >> 1 & 7)) << 4);
         }
     }
     __device__ __forceinline__ void issue(int i, int kb, uint8_t* image) const {
@@ -401,8 +402,8 @@ struct Piece {
     __device__ __forceinline__ Piece(int row, int g) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            x[h] = row * KB + (((4 * h + 2 * g) ^ (row & 7)) << 4);
-            y[h] = row * KB + (((4 * h + 2 * g + 1) ^ (row & 7)) << 4);
+            x[h] = row * KB + (((4 * h + 2 * g) ^ (row >> 1 & 7)) << 4);
+            y[h] = row * KB + (((4 * h + 2 * g + 1) ^ (row >> 1 & 7)) << 4);
         }
     }
     __device__ __forceinline__ i32x8 read(const uint8_t* image, int h, int t) const {      // of the row 32 t further (the order of its pieces is the same)

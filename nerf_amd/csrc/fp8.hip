@@ -361,12 +361,13 @@ __global__ void __launch_bounds__(64 * FEW_WAVES) k_product_few(Product p) {
 // ---- tiles --------------------------------------------------------------------------------------------------------------------
 // A workgroup of four waves owns a BM x BN tile of C, a wave a quarter of it in 32 x 32 pieces.  Per block of k, (BM + BN) rows of 128
 // bytes go from memory straight into LDS (global_load_lds, 16 bytes a lane), into one of two images.  A block is multiplied in two
-// halves of 64: while the first multiplies out of registers, the second's fragments are read, after which the image is done with:
-// behind the block's one barrier, while the second half multiplies, the rows of the block after the next are asked for in its place and
-// the first fragments of the next block are read.  So a request has one and a half blocks of multiplication to arrive and a
-// read half a block; neither is waited for.  The 16-byte pieces of a row are stored in the order piece ^ (row / 2 & 7): the sixteen
-// lanes whose 16-byte reads the LDS serves together hold rows that differ in this and the row's parity, so they cover all 64 banks
-// (piece ^ (row & 7) cost as many cycles again in conflicts).
+// halves of 64: while the first multiplies out of registers, the second's fragments are read, after which the image is done with;
+// from then on the rows of the block after the next are asked for in its place, one request beside each matrix instruction, and
+// while the second half multiplies, the first fragments of the next block are read.  So a request has a block of multiplication to
+// arrive and a read a quarter of one.  (The requests take half of the address path's time: all in one half block they held the matrix
+// instructions up, 8192^3 in 440 us against 416.)  The 16-byte pieces of a row are stored in the order piece ^ (row / 2 & 7): the
+// sixteen lanes whose 16-byte reads the LDS serves together hold rows that differ in this and the row's parity, so they cover all 64
+// banks (piece ^ (row & 7) cost as many cycles again in conflicts).
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ f32x16 mul32_fp8(i32x8 a, int sa, i32x8 b, int sb, f32x16 acc) {
@@ -551,9 +552,12 @@ __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, in
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto block = [&](int kb, auto more) {      // more: there are two blocks behind this one
-        constexpr int M = MT * NT, P = MT + NT;      // P <= M: a piece beside each of the first P
-        static_assert(P <= M);
+    constexpr int M = MT * NT, P = MT + NT;      // P <= M: a piece beside each of the first P
+    static_assert(P <= M);
+    constexpr bool LONG = M >= 16;               // half a block takes long enough for barriers of its own
+    constexpr int X = P + 1, Y = 3, EARLY = LONG ? M - 1 - X : 0, WORD_ISSUES = SROWS / 64;
+    auto block = [&](int kb, auto more) {        // more: there are two blocks behind this one
+        constexpr bool MORE = decltype(more)::value;
         const int sh = 8 * (kb & 3);
 #pragma unroll
         for (int t = 0; t < MT; ++t) wa[t] = na[t] >> sh;
@@ -561,18 +565,41 @@ __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, in
         for (int u = 0; u < NT; ++u) wb[u] = nb[u] >> sh;
         multiply(a0, b0, [&](int i) {
             if (i < P) fetch(i, kb, 1, a1, b1);
-        });
-        // this wave's rows of the next block are in LDS, then everyone's; and everyone is done with this one's image
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(a1, b1, [&](int i) {
-            if constexpr (decltype(more)::value) {
-                if (i == 0) issue_words((kb + 2) >> 2);
-#pragma unroll
-                for (int q = i * N / M; q < (i + 1) * N / M; ++q) issue(q, kb + 2);
+            if constexpr (LONG) {
+                if (i == X) {      // everyone is done with this block's image
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    if constexpr (MORE) issue_words((kb + 2) >> 2);
+                }
+                if constexpr (MORE) {
+                    if (i > X) issue(i - X - 1, kb + 2);
+                }
             }
-            if (i < P) fetch(i, kb + 1, 0, a0, b0);
-            if (i == M / 2) fetch_words(kb + 1);
+        });
+        if constexpr (!LONG) {
+            // this wave's rows of the next block are in LDS, then everyone's; and everyone is done with this one's image
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        multiply(a1, b1, [&](int i) {
+            if constexpr (LONG) {
+                if constexpr (MORE) {
+                    if (EARLY + i < N) issue(EARLY + i, kb + 2);
+                }
+                if (i == Y) {      // the next block is in LDS, all but what was asked for since
+                    if constexpr (MORE) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(WORD_ISSUES + EARLY + Y + 1) : "memory");
+                    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+                }
+                if (i > Y && i - Y - 1 < P) fetch(i - Y - 1, kb + 1, 0, a0, b0);
+                if (i == Y + P + 1) fetch_words(kb + 1);
+            } else {
+                if constexpr (MORE) {
+                    if (i == 0) issue_words((kb + 2) >> 2);
+#pragma unroll
+                    for (int q = i * N / M; q < (i + 1) * N / M; ++q) issue(q, kb + 2);
+                }
+                if (i < P) fetch(i, kb + 1, 0, a0, b0);
+                if (i == M / 2) fetch_words(kb + 1);
+            }
         });
     };
     issue_words(kb0 >> 2);

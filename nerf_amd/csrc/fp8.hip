@@ -381,7 +381,8 @@ struct Stage {      // one operand's rows on their way into LDS
     static constexpr int N = ROWS / 32;      // instructions of a wave per block, eight rows each
     const uint8_t* base;
     unsigned offset[N];      // of this lane's 16 bytes; rows behind the last stand for the last
-    __device__ __forceinline__ Stage(const uint8_t* p, int64_t row0, int64_t rows, int64_t ldk) : base(p + row0 * ldk) {
+    __device__ __forceinline__ void aim(const uint8_t* p, int64_t row0, int64_t rows, int64_t ldk) {
+        base = p + row0 * ldk;
         const int lane = threadIdx.x & 63, wave = wave_id();
         const int last = (int)(rows - row0 < ROWS ? rows - row0 : ROWS) - 1;
         const int r = lane >> 3;
@@ -413,120 +414,166 @@ struct Piece {
     }
 };
 
-// 32 rows x COLS columns of a wave's LDS image to out[row][col], each lane 16 bytes of a row at a time
+// eight rows x COLS columns of a wave's LDS band to out[row][col], each lane 16 bytes of a row at a time
 template <typename T, int COLS, int LD>
-__device__ __forceinline__ void emit(const float* image, const Product& p, int64_t row0, int64_t col0, T* out, int64_t ldo, bool wide, bool last) {
-    constexpr int VEC = 16 / sizeof(T), GROUPS = COLS / VEC, ROWS = 64 / GROUPS;
-    const int lane = threadIdx.x & 63;
-    const int c = (lane % GROUPS) * VEC, rl = lane / GROUPS;
-    const int64_t col = col0 + c;
-    if (col >= p.n) return;
-    const bool whole = wide && col + VEC <= p.n;
-    float bias[VEC];
+struct Out {
+    static constexpr int VEC = 16 / sizeof(T), GROUPS = COLS / VEC, ROWS = 64 / GROUPS;
+    static_assert(8 % ROWS == 0);
+    T* out;
+    const float* from;
+    int64_t m, ldo;
+    int rl, cols;      // cols of this lane's VEC are in the matrix
+    bool whole;
+    float floor, bias[VEC];
+    __device__ __forceinline__ Out(const float* band, const Product& p, int64_t col0, T* o, int64_t ld, bool wide, bool last) : m(p.m), ldo(ld) {
+        const int lane = threadIdx.x & 63, c = (lane % GROUPS) * VEC;
+        const int64_t col = col0 + c;
+        rl = lane / GROUPS;
+        from = band + rl * LD + c;
+        out = o + col;
+        cols = col + VEC <= p.n ? VEC : (col < p.n ? (int)(p.n - col) : 0);
+        whole = wide && cols == VEC;
+        floor = last && p.relu ? 0.0f : -INFINITY;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e)
-        bias[e] = last && p.bias && col + e < p.n ? (p.bias_f32 ? ((const float*)p.bias)[col + e] : (float)((const T*)p.bias)[col + e]) : 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < 32 / ROWS; ++i) {
-        const int64_t row = row0 + i * ROWS + rl;
-        if (row >= p.m) break;
-        float v[VEC];
+        for (int e = 0; e < VEC; ++e) bias[e] = 0.0f;
+        auto take = [&](const auto* b) {
 #pragma unroll
-        for (int e = 0; e < VEC; e += 4) {
-            const float4 q = *reinterpret_cast<const float4*>(image + (i * ROWS + rl) * LD + c + e);
-            v[e] = q.x; v[e + 1] = q.y; v[e + 2] = q.z; v[e + 3] = q.w;
-        }
-        if (last) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                v[e] += bias[e];
-                if (p.relu) v[e] = v[e] > 0.0f ? v[e] : (v[e] != v[e] ? v[e] : 0.0f);      // keeps a NaN
-            }
-        }
-        T* dst = out + row * ldo + col;
-        if (whole) {
-            store_vec<T, VEC>(dst, v);
-        } else {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e)
-                if (col + e < p.n) dst[e] = (T)v[e];
+            for (int e = 0; e < VEC; ++e) bias[e] = (float)b[col + e < p.n ? col + e : p.n - 1];
+        };
+        if (last && p.bias) {
+            if (p.bias_f32) take((const float*)p.bias);
+            else take((const T*)p.bias);
         }
     }
-}
+    // WHOLE: the wave's rows and columns are all in the matrix, and 16 bytes of a row are aligned
+    template <bool WHOLE>
+    __device__ __forceinline__ void rows(int64_t row0) const {
+        constexpr int R = 8 / ROWS;
+        float v[R][VEC];
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; e += 4) {
+                const f32x4 q = *reinterpret_cast<const f32x4*>(from + i * ROWS * LD + e);
+#pragma unroll
+                for (int d = 0; d < 4; ++d) v[i][e + d] = q[d];
+            }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                v[i][e] += bias[e];
+                v[i][e] = v[i][e] < floor ? 0.0f : v[i][e];      // keeps a NaN
+            }
+            const int64_t row = row0 + i * ROWS + rl;
+            T* dst = out + row * ldo;
+            if (WHOLE) {
+                store_vec<T, VEC>(dst, v[i]);
+            } else if (row < m) {
+                if (whole) {
+                    store_vec<T, VEC>(dst, v[i]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e)
+                        if (e < cols) dst[e] = (T)v[i][e];
+                }
+            }
+        }
+    }
+};
 
+template <typename T, int BM, int BN>
+struct TileLds {      // two images, two sets of scale words, a band of eight rows for each wave on its way out
+    static constexpr int IMAGE = (BM + BN) * KB, WORDS = (BM + BN) * 4, LD = BN / 2 + 4, BAND = 8 * LD * 4;
+    static constexpr int WORDS_AT = 2 * IMAGE, BAND_AT = WORDS_AT + 2 * WORDS, BYTES = BAND_AT + 4 * BAND;
+};
+
+// A workgroup stays for several tiles, and k runs on from one into the next: the requests for a tile's first blocks go out while the
+// one before it is still multiplied and written.  (A workgroup for each tile spent 11.5 us of 103 on the way out and in; bf16 of
+// 8192^3: 413 -> 390 us, 16384 x 8192 x 4096: 462 -> 409 us.)
 template <typename T, int BM, int BN>
 __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, int tiles_n, int blocks_per_slice, float* __restrict__ partial) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int MT = BM / 64, NT = BN / 64;      // 32 x 32 pieces of a wave
+    constexpr int M = MT * NT, P = MT + NT;        // P <= M: a piece beside each of the first P
+    static_assert(P <= M);
+    constexpr bool LONG = M >= 16;                 // half a block takes long enough for barriers of its own
+    using Lds = TileLds<T, BM, BN>;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = wave_id(), r = lane & 31, g = lane >> 5;
-    // neighbouring tiles on one XCD (workgroups go to the eight XCDs in turn), in bands of four rows of tiles
-    int id = blockIdx.x;
     const int total = tiles_m * tiles_n;
-    {
-        const int per = total / 8, extra = total % 8, x = id & 7, y = id >> 3;
-        id = x * per + (x < extra ? x : extra) + y;
-    }
-    constexpr int BAND = 4;
-    const int band = id / (BAND * tiles_n), in_band = id - band * BAND * tiles_n;
-    const int band_rows = tiles_m - band * BAND < BAND ? tiles_m - band * BAND : BAND;
-    const int64_t i0 = (int64_t)(band * BAND + in_band % band_rows) * BM, j0 = (int64_t)(in_band / band_rows) * BN;
     const int kb0 = blockIdx.z * blocks_per_slice;
     const int kb1 = kb0 + blocks_per_slice < p.blocks ? kb0 + blocks_per_slice : p.blocks;
-
-    const Stage<BM> sa(p.a, i0, p.m, p.ldk);
-    const Stage<BN> sb(p.b, j0, p.n, p.ldk);
     const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
-    f32x16 acc[MT][NT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int u = 0; u < NT; ++u)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[t][u][e] = 0.0f;
 
-    constexpr int IMAGE = (BM + BN) * KB, WORDS = (BM + BN) * 4;
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];      // two images, two sets of scale words
-    // the scales of four blocks are a word per row; a set of words comes along with the first image that needs it
-    constexpr int SROWS = (BM + BN) / 4;      // rows of a wave
-    const uint8_t* srow[SROWS / 64];
+    // neighbouring tiles on one XCD (workgroups go to the eight XCDs in turn), in bands of four rows of tiles
+    auto corner = [&](int id, int64_t& i0, int64_t& j0) {
+        constexpr int BAND = 4;
+        const int per = total / 8, extra = total % 8, x = id & 7;
+        id = x * per + (x < extra ? x : extra) + (id >> 3);
+        const int band = id / (BAND * tiles_n), in_band = id - band * BAND * tiles_n;
+        const int band_rows = tiles_m - band * BAND < BAND ? tiles_m - band * BAND : BAND;
+        i0 = (int64_t)(band * BAND + in_band % band_rows) * BM;
+        j0 = (int64_t)(in_band / band_rows) * BN;
+    };
+
+    // requests: the rows of one operand each, and the scales, four blocks' a word per row, which come along with every block
+    constexpr int SROWS = (BM + BN) / 4, WORD_ISSUES = SROWS / 64;      // rows of a wave
+    Stage<BM> sa;
+    Stage<BN> sb;
+    const uint8_t* srow[WORD_ISSUES];
+    auto aim = [&](int64_t i0, int64_t j0) {
+        sa.aim(p.a, i0, p.m, p.ldk);
+        sb.aim(p.b, j0, p.n, p.ldk);
 #pragma unroll
-    for (int i = 0; i < SROWS / 64; ++i) {
-        const int row = SROWS * wave + 64 * i + lane;      // A's rows, then B's
-        if (SROWS * wave + 64 * i < BM) srow[i] = p.sa + (i0 + row < p.m ? i0 + row : p.m - 1) * p.lds;
-        else srow[i] = p.sb + (j0 + row - BM < p.n ? j0 + row - BM : p.n - 1) * p.lds;
-    }
-    uint8_t* const words = lds + 2 * IMAGE;
-    auto issue_words = [&](int group) {
-#pragma unroll
-        for (int i = 0; i < SROWS / 64; ++i)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(srow[i] + 4 * (int64_t)group),
-                                             (__attribute__((address_space(3))) void*)(words + (group & 1) * WORDS + (SROWS * wave + 64 * i) * 4), 4, 0, 0);
+        for (int i = 0; i < WORD_ISSUES; ++i) {
+            const int row = SROWS * wave + 64 * i + lane;      // A's rows, then B's
+            if (SROWS * wave + 64 * i < BM) srow[i] = p.sa + (i0 + row < p.m ? i0 + row : p.m - 1) * p.lds;
+            else srow[i] = p.sb + (j0 + row - BM < p.n ? j0 + row - BM : p.n - 1) * p.lds;
+        }
     };
     constexpr int NA = Stage<BM>::N, N = NA + Stage<BN>::N;      // this wave's row instructions of a block
-    auto issue = [&](int i, int kb) {
-        uint8_t* image = lds + (kb & 1) * IMAGE;
+    auto issue = [&](int i, int kb, int place) {
+        uint8_t* image = lds + place * Lds::IMAGE;
         if (i < NA) sa.issue(i, kb, image);
         else sb.issue(i - NA, kb, image + BM * KB);
     };
+    auto issue_words = [&](int kb, int place) {
+#pragma unroll
+        for (int i = 0; i < WORD_ISSUES; ++i)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(srow[i] + 4 * (int64_t)(kb >> 2)),
+                                             (__attribute__((address_space(3))) void*)(lds + Lds::WORDS_AT + place * Lds::WORDS + (SROWS * wave + 64 * i) * 4), 4, 0, 0);
+    };
+
+    // reads
     const Piece pa(wm + r, g), pb(wn + r, g);
     i32x8 a0[MT], b0[NT], a1[MT], b1[NT];
     unsigned wa[MT], wb[NT], na[MT], nb[NT];
-    auto fetch = [&](int i, int kb, int h, i32x8 (&a)[MT], i32x8 (&b)[NT]) {      // piece i of a half block's MT + NT
-        const uint8_t* image = lds + (kb & 1) * IMAGE;
+    auto fetch = [&](int i, int place, int h, i32x8 (&a)[MT], i32x8 (&b)[NT]) {      // piece i of a half block's MT + NT
+        const uint8_t* image = lds + place * Lds::IMAGE;
         if (i < MT) a[i] = pa.read(image, h, i);
         else b[i - MT] = pb.read(image + BM * KB, h, i - MT);
     };
-    auto fetch_words = [&](int kb) {
-        const unsigned* w = reinterpret_cast<const unsigned*>(words + ((kb >> 2) & 1) * WORDS);
+    auto fetch_words = [&](int place) {
+        const unsigned* w = reinterpret_cast<const unsigned*>(lds + Lds::WORDS_AT + place * Lds::WORDS);
 #pragma unroll
         for (int t = 0; t < MT; ++t) na[t] = w[wm + 32 * t + r];
 #pragma unroll
         for (int u = 0; u < NT; ++u) nb[u] = w[BM + wn + 32 * u + r];
     };
+
+    f32x16 acc[MT][NT];
+    auto clear = [&] {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[t][u][e] = 0.0f;
+    };
     // One half block multiplies out of a, b; between its instructions and in this order `beside(i)` places reads and requests.  (One wave
     // per SIMD: what is not placed between matrix instructions, which take 64 cycles each, is waited for.)
     auto multiply = [&](const i32x8 (&a)[MT], const i32x8 (&b)[NT], auto beside) {
-        constexpr int M = MT * NT;
         if constexpr (!F32) {
 #pragma unroll
             for (int i = 0; i < M; ++i) {
@@ -552,92 +599,140 @@ __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, in
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    constexpr int M = MT * NT, P = MT + NT;      // P <= M: a piece beside each of the first P
-    static_assert(P <= M);
-    constexpr bool LONG = M >= 16;               // half a block takes long enough for barriers of its own
-    constexpr int X = P + 1, Y = 3, EARLY = LONG ? M - 1 - X : 0, WORD_ISSUES = SROWS / 64;
-    auto block = [&](int kb, auto more) {        // more: there are two blocks behind this one
-        constexpr bool MORE = decltype(more)::value;
+    auto scales_of = [&](int kb) {
         const int sh = 8 * (kb & 3);
 #pragma unroll
         for (int t = 0; t < MT; ++t) wa[t] = na[t] >> sh;
 #pragma unroll
         for (int u = 0; u < NT; ++u) wb[u] = nb[u] >> sh;
-        multiply(a0, b0, [&](int i) {
-            if (i < P) fetch(i, kb, 1, a1, b1);
-            if constexpr (LONG) {
-                if (i == X) {      // everyone is done with this block's image
-                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                    if constexpr (MORE) issue_words((kb + 2) >> 2);
-                }
-                if constexpr (MORE) {
-                    if (i > X) issue(i - X - 1, kb + 2);
-                }
+    };
+    // out through LDS, eight rows of the wave's columns at a time, so that a store is 16 bytes of a row (or fp32 partial sums likewise)
+    float* const band = reinterpret_cast<float*>(lds + Lds::BAND_AT) + wave * 8 * Lds::LD;
+    auto write_by = [&](const auto& out, int64_t i0, auto whole) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+#pragma unroll
+                for (int u = 0; u < NT; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) band[(e + 4 * g) * Lds::LD + 32 * u + r] = acc[t][u][4 * q + e];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // (one wave's LDS instructions run in order)
+                out.template rows<decltype(whole)::value>(i0 + wm + 32 * t + 8 * q);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             }
-        });
-        if constexpr (!LONG) {
+    };
+    auto write = [&](int64_t i0, int64_t j0) {
+        if (!LONG && partial) {
+            write_by(Out<float, 32 * NT, Lds::LD>(band, p, j0 + wn, partial + (int64_t)blockIdx.z * p.m * p.n, p.n, (p.n & 3) == 0, false), i0, std::false_type{});
+        } else {
+            const Out<T, 32 * NT, Lds::LD> out(band, p, j0 + wn, (T*)p.c, p.ldc, p.wide != 0, true);
+            if (i0 + BM <= p.m && j0 + BN <= p.n && p.wide) write_by(out, i0, std::true_type{});
+            else write_by(out, i0, std::false_type{});
+        }
+    };
+
+    int64_t i0, j0;
+    corner(blockIdx.x, i0, j0);
+    aim(i0, j0);
+    clear();
+    if constexpr (LONG) {
+        constexpr int X = P + 1, Y = 3, EARLY = M - 1 - X;
+        // The block asked for runs two ahead of the one multiplied, into the next tile where this one ends.  Behind the last it stays
+        // where it is: its rows come once more, for nobody.
+        int ask_tile = blockIdx.x, ask_kb = kb0, ask_words = 0, ask_image = 0;
+        auto ask_next = [&] {
+            ask_image ^= 1;
+            if (ask_kb + 1 < kb1) {
+                ++ask_kb;
+                if ((ask_kb & 3) == 0) ask_words ^= 1;
+            } else if (ask_tile + (int)gridDim.x < total) {
+                ask_tile += gridDim.x;
+                ask_kb = kb0;
+                ask_words ^= 1;
+                int64_t i, j;
+                corner(ask_tile, i, j);
+                aim(i, j);
+            }
+        };
+        auto ask_all = [&] {
+            issue_words(ask_kb, ask_words);
+#pragma unroll
+            for (int i = 0; i < N; ++i) issue(i, ask_kb, ask_image);
+        };
+        ask_all();
+        ask_next();
+        ask_all();
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N + WORD_ISSUES) : "memory");
+#pragma unroll
+        for (int i = 0; i < P; ++i) fetch(i, 0, 0, a0, b0);
+        fetch_words(0);
+        int image = 0, set = 0;
+        for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
+            for (int kb = kb0; kb < kb1; ++kb) {
+                ask_next();
+                scales_of(kb);
+                multiply(a0, b0, [&](int i) {
+                    if (i < P) fetch(i, image, 1, a1, b1);
+                    if (i == X) {      // everyone is done with this block's image
+                        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                        issue_words(ask_kb, ask_words);
+                    }
+                    if (i > X) issue(i - X - 1, ask_kb, ask_image);
+                });
+                // (the next block's scales are in the other set where a new word begins: four blocks on, or in another tile)
+                if (kb + 1 == kb1 || ((kb + 1) & 3) == 0) set ^= 1;
+                image ^= 1;
+                multiply(a1, b1, [&](int i) {
+                    if (EARLY + i < N) issue(EARLY + i, ask_kb, ask_image);
+                    if (i == Y)      // the next block is in LDS: out are at most the requests made since
+                        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(WORD_ISSUES + EARLY + Y + 1) : "memory");
+                    if (i > Y && i - Y - 1 < P) fetch(i - Y - 1, image, 0, a0, b0);
+                    if (i == Y + P + 1) fetch_words(set);
+                });
+            }
+            corner(tile, i0, j0);
+            write(i0, j0);
+            clear();
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // nothing may arrive in LDS that is another workgroup's by then
+    } else {
+        auto place_of = [&](int kb) { return (kb >> 2) & 1; };
+        auto block = [&](int kb, auto more) {      // more: there are two blocks behind this one
+            scales_of(kb);
+            multiply(a0, b0, [&](int i) { if (i < P) fetch(i, kb & 1, 1, a1, b1); });
             // this wave's rows of the next block are in LDS, then everyone's; and everyone is done with this one's image
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             __builtin_amdgcn_sched_barrier(0);
+            multiply(a1, b1, [&](int i) {
+                if constexpr (decltype(more)::value) {
+                    if (i == 0) issue_words(kb + 2, place_of(kb + 2));
+#pragma unroll
+                    for (int q = i * N / M; q < (i + 1) * N / M; ++q) issue(q, kb + 2, kb & 1);
+                }
+                if (i < P) fetch(i, (kb + 1) & 1, 0, a0, b0);
+                if (i == M / 2) fetch_words(place_of(kb + 1));
+            });
+        };
+        issue_words(kb0, place_of(kb0));
+#pragma unroll
+        for (int i = 0; i < N; ++i) issue(i, kb0, kb0 & 1);
+        if (kb0 + 1 < kb1) {
+            issue_words(kb0 + 1, place_of(kb0 + 1));
+#pragma unroll
+            for (int i = 0; i < N; ++i) issue(i, kb0 + 1, (kb0 + 1) & 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
-        multiply(a1, b1, [&](int i) {
-            if constexpr (LONG) {
-                if constexpr (MORE) {
-                    if (EARLY + i < N) issue(EARLY + i, kb + 2);
-                }
-                if (i == Y) {      // the next block is in LDS, all but what was asked for since
-                    if constexpr (MORE) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(WORD_ISSUES + EARLY + Y + 1) : "memory");
-                    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-                }
-                if (i > Y && i - Y - 1 < P) fetch(i - Y - 1, kb + 1, 0, a0, b0);
-                if (i == Y + P + 1) fetch_words(kb + 1);
-            } else {
-                if constexpr (MORE) {
-                    if (i == 0) issue_words((kb + 2) >> 2);
+        asm volatile("s_barrier" ::: "memory");
 #pragma unroll
-                    for (int q = i * N / M; q < (i + 1) * N / M; ++q) issue(q, kb + 2);
-                }
-                if (i < P) fetch(i, kb + 1, 0, a0, b0);
-                if (i == M / 2) fetch_words(kb + 1);
-            }
-        });
-    };
-    issue_words(kb0 >> 2);
-#pragma unroll
-    for (int i = 0; i < N; ++i) issue(i, kb0);
-    if (kb0 + 1 < kb1) {
-        issue_words((kb0 + 1) >> 2);
-#pragma unroll
-        for (int i = 0; i < N; ++i) issue(i, kb0 + 1);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-    } else {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
-    asm volatile("s_barrier" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < MT + NT; ++i) fetch(i, kb0, 0, a0, b0);
-    fetch_words(kb0);
-    int kb = kb0;
-    for (; kb + 2 < kb1; ++kb) block(kb, std::true_type{});
-    for (; kb < kb1; ++kb) block(kb, std::false_type{});      // (behind the last block an image's old rows are read and not used)
-    // out through LDS, 32 rows of the wave's columns at a time, so that a store is 16 bytes of a row (or fp32 partial sums likewise)
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    asm volatile("s_barrier" ::: "memory");
-    constexpr int COLS = 32 * NT, LD = COLS + 4;
-    static_assert(4 * 32 * LD * sizeof(float) <= 2 * IMAGE, "the bands of four waves lie in the images");
-    float* band_image = reinterpret_cast<float*>(lds) + wave * 32 * LD;
-    const bool sums = partial != nullptr;
-    const int64_t col0 = j0 + wn;
-    float* part = sums ? partial + (int64_t)blockIdx.z * p.m * p.n : nullptr;
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-#pragma unroll
-        for (int u = 0; u < NT; ++u)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) band_image[((e & 3) + 8 * (e >> 2) + 4 * g) * LD + 32 * u + r] = acc[t][u][e];
-        const int64_t row0 = i0 + wm + 32 * t;
-        if (sums) emit<float, COLS, LD>(band_image, p, row0, col0, part, p.n, (p.n & 3) == 0, false);
-        else emit<T, COLS, LD>(band_image, p, row0, col0, (T*)p.c, p.ldc, p.wide != 0, true);
+        for (int i = 0; i < P; ++i) fetch(i, kb0 & 1, 0, a0, b0);
+        fetch_words(place_of(kb0));
+        int kb = kb0;
+        for (; kb + 2 < kb1; ++kb) block(kb, std::true_type{});
+        for (; kb < kb1; ++kb) block(kb, std::false_type{});      // (behind the last block an image's old rows are read and not used)
+        write(i0, j0);
     }
 }
 
@@ -686,20 +781,21 @@ struct Plan {
     int tile;           // 0: few rows; else the tile's edge
     int slices;         // of k
     int blocks_per_slice;
+    int units;          // compute units: workgroups that stay for several large tiles
 };
 Plan plan_of(int64_t m, int64_t n, int64_t k, int type) {
     const int64_t blocks = blocks_of(k);
-    if (m <= 64 || k > (1 << 22)) return {0, 1, (int)blocks};
+    if (m <= 64 || k > (1 << 22)) return {0, 1, (int)blocks, 0};
     auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
     const int cus = 256;
     const int tile = type != NERF_F32 && tiles(256) >= cus ? 256 : 128;
     int64_t slices = 1;
-    const int64_t count = tiles(tile);
+    const int64_t count = tiles(tile);      // (large tiles are never sliced)
     if (count < cus) slices = cus / count;
     if (slices > blocks / 4) slices = blocks / 4;
     if (slices < 1) slices = 1;
     const int64_t per = (blocks + slices - 1) / slices;
-    return {tile, (int)((blocks + per - 1) / per), (int)per};
+    return {tile, (int)((blocks + per - 1) / per), (int)per, cus};
 }
 
 template <typename T>
@@ -716,12 +812,13 @@ int product(const Product& p, int64_t k, int type, float* ws, hipStream_t stream
     }
     const int64_t tm = (p.m + plan.tile - 1) / plan.tile, tn = (p.n + plan.tile - 1) / plan.tile;
     if (tm * tn > 0xffffff) return fail(NERF_E_ARG, "nerf_fp8_matmul: %lld x %lld is more than one launch covers", (long long)p.m, (long long)p.n);
-    const dim3 grid((unsigned)(tm * tn), 1, (unsigned)plan.slices);
+    const int64_t wgs = plan.tile == 256 && tm * tn > plan.units ? plan.units : tm * tn;
+    const dim3 grid((unsigned)wgs, 1, (unsigned)plan.slices);
     float* part = plan.slices > 1 ? ws : nullptr;
     if (plan.slices > 1 && !ws) return fail(NERF_E_ARG, "nerf_fp8_matmul: null workspace");
 #define GO(E)                                                                                                                        \
     do {                                                                                                                             \
-        constexpr size_t bytes = (E + E) * (2 * KB + 8);                                                                                 \
+        constexpr size_t bytes = TileLds<T, E, E>::BYTES; \
         const hipError_t e = lds_limit_once((const void*)&k_product_tile<T, E, E>, bytes);                                           \
         if (e != hipSuccess) return fail(NERF_E_LAUNCH, "nerf_fp8_matmul: %s", hipGetErrorString(e));                                \
         hipLaunchKernelGGL((k_product_tile<T, E, E>), grid, dim3(256), bytes, stream, p, (int)tm, (int)tn, plan.blocks_per_slice, part); \

@@ -190,8 +190,11 @@ __global__ void __launch_bounds__(THREADS) k_adamw(Tensors ts, const Coef* __res
     }
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-        m[e] = m[e] + w1 * (g[e] - m[e]);
-        v[e] = v[e] + w2 * (g[e] * g[e] - v[e]);
+        {      // (each operation rounded by itself: with states in 8 bits a last place can move a code by a whole step)
+#pragma clang fp contract(off)
+            m[e] = m[e] + w1 * (g[e] - m[e]);
+            v[e] = v[e] + w2 * (g[e] * g[e] - v[e]);
+        }
         const float denom = sqrtf(v[e]) * c.inv_sqrt_bc2 + eps;
         p[e] -= c.lr_wd * p[e] + c.step_size * m[e] / denom;
     }
@@ -204,15 +207,15 @@ __global__ void __launch_bounds__(THREADS) k_adamw(Tensors ts, const Coef* __res
             am = mb > am ? mb : am;
             av = vb > av ? vb : av;
         }
-        const float sm = __uint_as_float(row_max(am)) / 448.0f, sv = __uint_as_float(row_max(av)) / 57344.0f;
-        const float im = 1.0f / fmaxf(sm, 1e-38f), iv = 1.0f / fmaxf(sv, 1e-38f);
+        const float sm = __uint_as_float(row_max(am)) * (1.0f / 448.0f), sv = __uint_as_float(row_max(av)) * (1.0f / 57344.0f);
+        const float dm = fmaxf(sm, 1e-38f), dv = fmaxf(sv, 1e-38f);
         unsigned a[2] = {0, 0}, b[2] = {0, 0};
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
             const unsigned h = noise(e0 + e, c.t);
-            unsigned cm = to_e4m3(fminf(fabsf(m[e]) * im, 448.0f), h & 0xffffu);
+            unsigned cm = to_e4m3(fminf(fabsf(m[e]) / dm, 448.0f), h & 0xffffu);
             cm |= (__float_as_uint(m[e]) >> 31) << 7;
-            unsigned cv = to_e5m2(fminf(v[e] * iv, 57344.0f), h >> 16);
+            unsigned cv = to_e5m2(fminf(v[e] / dv, 57344.0f), h >> 16);
             if (cv == 0 && v[e] > 0.0f) cv = 1;
             a[e >> 2] |= cm << (8 * (e & 3));
             b[e >> 2] |= cv << (8 * (e & 3));

@@ -785,7 +785,11 @@ struct Plan {
 };
 Plan plan_of(int64_t m, int64_t n, int64_t k, int type) {
     const int64_t blocks = blocks_of(k);
-    if (m <= 64 || k > (1 << 22)) return {0, 1, (int)blocks, 0};
+    // Few rows or tiles: what either takes in us, fitted to both at 4 to 64 rows and n x k from 256 x 256 to 8192 x 8192 and 1024 x 65536.
+    // (8192 x 8192: 4 rows 13.9 / 17.4, 16 rows 18.6 / 18.1, 64 rows 42.8 / 20.9; 1024 x 1024, 64 rows: 5.5 / 8.9;
+    // 1024 x 65536, 4 rows: 47 / 18, few workgroups with a long way each)
+    const double few = 2.4 + (double)k * (n > 4096 ? n : 4096) * (17 + m) / 1.34e8, many = 7.5 + (double)n * k / 6.4e6;
+    if ((m <= 64 && few <= many) || k > (1 << 22)) return {0, 1, (int)blocks, 0};
     auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
     const int cus = 256;
     const int tile = type != NERF_F32 && tiles(256) >= cus ? 256 : 128;

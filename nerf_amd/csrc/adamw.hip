@@ -92,8 +92,8 @@ __device__ __forceinline__ unsigned row_max(unsigned v) {
 }
 
 template <typename T>
-__device__ __forceinline__ void fetch(const T* p, int left, bool wide, float (&out)[PER]) {
-    if (wide && left >= PER) {
+__device__ __forceinline__ void fetch(const T* p, int left, float (&out)[PER]) {
+    if (left >= PER) {
         load_vec<T, PER>(p, out);
     } else {
 #pragma unroll
@@ -101,8 +101,8 @@ __device__ __forceinline__ void fetch(const T* p, int left, bool wide, float (&o
     }
 }
 template <typename T>
-__device__ __forceinline__ void put(T* p, int left, bool wide, const float (&in)[PER]) {
-    if (wide && left >= PER) {
+__device__ __forceinline__ void put(T* p, int left, const float (&in)[PER]) {
+    if (left >= PER) {
         store_vec<T, PER>(p, in);
     } else {
 #pragma unroll
@@ -110,11 +110,9 @@ __device__ __forceinline__ void put(T* p, int left, bool wide, const float (&in)
             if (e < left) p[e] = (T)in[e];
     }
 }
-__device__ __forceinline__ void fetch_codes(const uint8_t* p, int left, bool wide, unsigned (&w)[2]) {
-    if (wide && left >= PER) {
-        const uint2 q = *reinterpret_cast<const uint2*>(p);
-        w[0] = q.x;
-        w[1] = q.y;
+__device__ __forceinline__ void fetch_codes(const uint8_t* p, int left, unsigned (&w)[2]) {
+    if (left >= PER) {
+        __builtin_memcpy(w, p, PER);
     } else {
         w[0] = w[1] = 0;
 #pragma unroll
@@ -122,9 +120,9 @@ __device__ __forceinline__ void fetch_codes(const uint8_t* p, int left, bool wid
             if (e < left) w[e >> 2] |= (unsigned)p[e] << (8 * (e & 3));
     }
 }
-__device__ __forceinline__ void put_codes(uint8_t* p, int left, bool wide, const unsigned (&w)[2]) {
-    if (wide && left >= PER) {
-        *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+__device__ __forceinline__ void put_codes(uint8_t* p, int left, const unsigned (&w)[2]) {
+    if (left >= PER) {
+        __builtin_memcpy(p, w, PER);
     } else {
 #pragma unroll
         for (int e = 0; e < PER; ++e)
@@ -145,31 +143,25 @@ __global__ void __launch_bounds__(THREADS) k_adamw(Tensors ts, const Coef* __res
     T* pp = (T*)ts.p[i] + e0;
     const T* gp = (const T*)ts.g[i] + e0;
     float* masterp = NARROW ? ts.master[i] + e0 : nullptr;
-    uintptr_t bits = (uintptr_t)ts.p[i] | (uintptr_t)ts.g[i];
-    if (NARROW) bits |= (uintptr_t)ts.master[i];
-    if (!EIGHT) bits |= (uintptr_t)ts.m[i] | (uintptr_t)ts.v[i];
-    const bool wide = (bits & 15) == 0;
 
     float p[PER], g[PER], m[PER], v[PER];
-    fetch<T>(gp, left, wide, g);
-    fetch<T>(pp, left, wide, p);
+    fetch<T>(gp, left, g);
+    fetch<T>(pp, left, p);
     if (NARROW) {     // the master copy, unless the parameter was written since it was rounded from it
         float master[PER];
-        fetch<float>(masterp, left, wide, master);
+        fetch<float>(masterp, left, master);
 #pragma unroll
         for (int e = 0; e < PER; ++e) p[e] = (float)(T)master[e] == p[e] ? master[e] : p[e];
     }
     const int64_t block = (e0 >> 7);
     float *mp = nullptr, *vp = nullptr;
     uint8_t *mc = nullptr, *vc = nullptr;
-    bool wide8 = false;
     if (EIGHT) {
         mc = (uint8_t*)ts.m[i] + e0;
         vc = (uint8_t*)ts.v[i] + e0;
-        wide8 = (((uintptr_t)ts.m[i] | (uintptr_t)ts.v[i]) & 7) == 0;
         unsigned a[2], b[2];
-        fetch_codes(mc, left, wide8, a);
-        fetch_codes(vc, left, wide8, b);
+        fetch_codes(mc, left, a);
+        fetch_codes(vc, left, b);
         float sm = 0.0f, sv = 0.0f;
         if (left > 0) {
             sm = ts.scale[i][2 * block];
@@ -185,8 +177,8 @@ __global__ void __launch_bounds__(THREADS) k_adamw(Tensors ts, const Coef* __res
     } else {
         mp = (float*)ts.m[i] + e0;
         vp = (float*)ts.v[i] + e0;
-        fetch<float>(mp, left, wide, m);
-        fetch<float>(vp, left, wide, v);
+        fetch<float>(mp, left, m);
+        fetch<float>(vp, left, v);
     }
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
@@ -220,18 +212,18 @@ __global__ void __launch_bounds__(THREADS) k_adamw(Tensors ts, const Coef* __res
             a[e >> 2] |= cm << (8 * (e & 3));
             b[e >> 2] |= cv << (8 * (e & 3));
         }
-        put_codes(mc, left, wide8, a);
-        put_codes(vc, left, wide8, b);
+        put_codes(mc, left, a);
+        put_codes(vc, left, b);
         if (left > 0 && (threadIdx.x & 15) == 0) {
             ts.scale[i][2 * block] = sm;
             ts.scale[i][2 * block + 1] = sv;
         }
     } else {
-        put<float>(mp, left, wide, m);
-        put<float>(vp, left, wide, v);
+        put<float>(mp, left, m);
+        put<float>(vp, left, v);
     }
-    if (NARROW) put<float>(masterp, left, wide, p);
-    put<T>(pp, left, wide, p);
+    if (NARROW) put<float>(masterp, left, p);
+    put<T>(pp, left, p);
 }
 
 }  // namespace

@@ -19,24 +19,23 @@ template <> struct ElemTraits<f16_t> { static constexpr int code = 2; };
 inline int elem_size(int type) { return type == 0 ? 4 : 2; }
 inline bool elem_type_ok(int type) { return type >= 0 && type <= 2; }
 
-// N consecutive elements: one load or store of up to 16 bytes each; the address is a multiple of the vector's size (or of 16)
+// N consecutive elements from any element's address: the memory system takes vector accesses at any alignment, so that odd strides and
+// slices of larger buffers need no path of their own
 template <typename T, int N>
-struct __attribute__((aligned(sizeof(T) * N > 16 ? 16 : sizeof(T) * N))) Vec {
-    T e[N];
-};
+struct __attribute__((packed, aligned(sizeof(T)))) Loose { T e __attribute__((ext_vector_type(N))); };
 
 template <typename T, int N>
 __device__ __forceinline__ void load_vec(const T* p, float (&out)[N]) {
-    const Vec<T, N> v = *reinterpret_cast<const Vec<T, N>*>(p);
+    const Loose<T, N> v = *reinterpret_cast<const Loose<T, N>*>(p);
 #pragma unroll
     for (int i = 0; i < N; ++i) out[i] = (float)v.e[i];
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_vec(T* p, const float (&in)[N]) {
-    Vec<T, N> v;
+    Loose<T, N> v;
 #pragma unroll
     for (int i = 0; i < N; ++i) v.e[i] = (T)in[i];
-    *reinterpret_cast<Vec<T, N>*>(p) = v;
+    *reinterpret_cast<Loose<T, N>*>(p) = v;
 }
 
 }  // namespace nerfhip

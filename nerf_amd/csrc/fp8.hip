@@ -86,7 +86,7 @@ __device__ __forceinline__ void over_rows(unsigned (&v)[8], unsigned (*red)[QT],
 
 // Along the columns alone: sixteen lanes hold a block of 128, a workgroup 16 N blocks that follow one another in memory.
 template <typename T, int N>
-__global__ void __launch_bounds__(256) k_quantize_rows(int64_t rows, int64_t cols, const T* __restrict__ x, int64_t ldx, int wide,
+__global__ void __launch_bounds__(256) k_quantize_rows(int64_t rows, int64_t cols, const T* __restrict__ x, int64_t ldx,
                                                        unsigned blocks, uint8_t* __restrict__ codes, int64_t ldc, uint8_t* __restrict__ scales,
                                                        int64_t lds) {
     const int l = threadIdx.x & 15;
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(256) k_quantize_rows(int64_t rows, int64_t col
         row[q] = total <= 0xffffffffll ? (int64_t)((unsigned)id / blocks) : id / blocks;
         kb[q] = (unsigned)(id - row[q] * blocks);
         const int64_t c = (int64_t)kb[q] * KB + l * 8;
-        if (wide && row[q] < rows && c + 8 <= cols) {
+        if (row[q] < rows && c + 8 <= cols) {
             load_vec<T, 8>(x + row[q] * ldx + c, v[q]);
         } else {
 #pragma unroll
@@ -129,8 +129,8 @@ __global__ void __launch_bounds__(256) k_quantize_rows(int64_t rows, int64_t col
 // tile's columns, [tile row][cols].  mask: values whose mask entry is <= 0 count as 0 (the gradient of a ReLU's output).
 // One pass over x whatever is asked for; the transposed codes are packed along the rows in registers and cross the workgroup as bytes.
 template <typename T, bool ROWS>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) k_quantize(int64_t rows, int64_t cols, unsigned col_tiles, const T* __restrict__ x, int64_t ldx, int wide,
-                                                  const T* __restrict__ mask, int64_t ldm, int wide_mask, uint8_t* __restrict__ codes, int64_t ldc,
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) k_quantize(int64_t rows, int64_t cols, unsigned col_tiles, const T* __restrict__ x, int64_t ldx,
+                                                  const T* __restrict__ mask, int64_t ldm, uint8_t* __restrict__ codes, int64_t ldc,
                                                   uint8_t* __restrict__ scales, int64_t lds, uint8_t* __restrict__ codes_t, int64_t ldct,
                                                   uint8_t* __restrict__ scales_t, int64_t ldst, float* __restrict__ colsum) {
     const unsigned row_tile = blockIdx.x / col_tiles, col_tile = blockIdx.x - row_tile * col_tiles, row_tiles = gridDim.x / col_tiles;
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) k_quantize(int64_
     const int tid = threadIdx.x, rl = (tid >> 4) * 8, cl = (tid & 15) * 8;
     const int64_t c = c0 + cl;
     float v[8][8];
-    const bool inside = wide && r0 + QT <= rows && c0 + QT <= cols;      // of the whole tile
+    const bool inside = r0 + QT <= rows && c0 + QT <= cols;      // the whole tile
     const int nr = (int)(rows - r0 - rl < 8 ? rows - r0 - rl : 8), nc = (int)(cols - c < 8 ? cols - c : 8);      // this thread's valid part, possibly < 1
     const T* src = x + (r0 + rl) * ldx + c;
     if (inside) {
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) k_quantize(int64_
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
             float m[8];
-            if (inside && wide_mask) {
+            if (inside) {
                 load_vec<T, 8>(gate + q * ldm, m);
             } else {
 #pragma unroll
@@ -263,7 +263,6 @@ struct Product {
     int bias_f32, relu;
     void* c;
     int64_t ldc;
-    int wide;                 // rows of c start at multiples of 16 bytes
 };
 
 template <typename T>
@@ -423,16 +422,14 @@ struct Out {
     const float* from;
     int64_t m, ldo;
     int rl, cols;      // cols of this lane's VEC are in the matrix
-    bool whole;
     float floor, bias[VEC];
-    __device__ __forceinline__ Out(const float* band, const Product& p, int64_t col0, T* o, int64_t ld, bool wide, bool last) : m(p.m), ldo(ld) {
+    __device__ __forceinline__ Out(const float* band, const Product& p, int64_t col0, T* o, int64_t ld, bool last) : m(p.m), ldo(ld) {
         const int lane = threadIdx.x & 63, c = (lane % GROUPS) * VEC;
         const int64_t col = col0 + c;
         rl = lane / GROUPS;
         from = band + rl * LD + c;
         out = o + col;
         cols = col + VEC <= p.n ? VEC : (col < p.n ? (int)(p.n - col) : 0);
-        whole = wide && cols == VEC;
         floor = last && p.relu ? 0.0f : -INFINITY;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) bias[e] = 0.0f;
@@ -445,7 +442,7 @@ struct Out {
             else take((const T*)p.bias);
         }
     }
-    // WHOLE: the wave's rows and columns are all in the matrix, and 16 bytes of a row are aligned
+    // WHOLE: the wave's rows and columns are all in the matrix
     template <bool WHOLE>
     __device__ __forceinline__ void rows(int64_t row0) const {
         constexpr int R = 8 / ROWS;
@@ -470,7 +467,7 @@ struct Out {
             if (WHOLE) {
                 store_vec<T, VEC>(dst, v[i]);
             } else if (row < m) {
-                if (whole) {
+                if (cols == VEC) {
                     store_vec<T, VEC>(dst, v[i]);
                 } else {
 #pragma unroll
@@ -624,10 +621,10 @@ __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, in
     };
     auto write = [&](int64_t i0, int64_t j0) {
         if (!LONG && partial) {
-            write_by(Out<float, 32 * NT, Lds::LD>(band, p, j0 + wn, partial + (int64_t)blockIdx.z * p.m * p.n, p.n, (p.n & 3) == 0, false), i0, std::false_type{});
+            write_by(Out<float, 32 * NT, Lds::LD>(band, p, j0 + wn, partial + (int64_t)blockIdx.z * p.m * p.n, p.n, false), i0, std::false_type{});
         } else {
-            const Out<T, 32 * NT, Lds::LD> out(band, p, j0 + wn, (T*)p.c, p.ldc, p.wide != 0, true);
-            if (i0 + BM <= p.m && j0 + BN <= p.n && p.wide) write_by(out, i0, std::true_type{});
+            const Out<T, 32 * NT, Lds::LD> out(band, p, j0 + wn, (T*)p.c, p.ldc, true);
+            if (i0 + BM <= p.m && j0 + BN <= p.n) write_by(out, i0, std::true_type{});
             else write_by(out, i0, std::false_type{});
         }
     };
@@ -843,14 +840,12 @@ template <typename T>
 int quantize(int64_t rows, int64_t cols, const T* x, int64_t ldx, const T* mask, int64_t ldm, uint8_t* codes, uint8_t* scales,
              uint8_t* codes_t, uint8_t* scales_t, int sum_type, void* col_sum, float* ws, hipStream_t stream) {
     const int64_t ldc = code_stride(cols), lds = scale_stride(cols), ldct = code_stride(rows), ldst = scale_stride(rows);
-    const int wide = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(ldx * sizeof(T))) & 15) == 0;
-    const int wide_mask = ((reinterpret_cast<uintptr_t>(mask) | (uintptr_t)(ldm * sizeof(T))) & 15) == 0;
     if (codes_t || col_sum || mask) {
         const int64_t col_tiles = (cols + QT - 1) / QT, tiles_all = (rows + QT - 1) / QT * col_tiles;
         if (tiles_all > 0xffffff) return fail(NERF_E_ARG, "nerf_fp8_quantize: %lld x %lld is more than one launch covers", (long long)rows, (long long)cols);
 #define GO(R)                                                                                                                        \
-    hipLaunchKernelGGL((k_quantize<T, R>), dim3((unsigned)tiles_all), dim3(256), 0, stream, rows, cols, (unsigned)col_tiles, x, ldx, wide, mask, \
-                       ldm, wide_mask, codes, ldc, scales, lds, codes_t, ldct, scales_t, ldst, col_sum ? ws : (float*)nullptr)
+    hipLaunchKernelGGL((k_quantize<T, R>), dim3((unsigned)tiles_all), dim3(256), 0, stream, rows, cols, (unsigned)col_tiles, x, ldx, mask, ldm, \
+                       codes, ldc, scales, lds, codes_t, ldct, scales_t, ldst, col_sum ? ws : (float*)nullptr)
         if (codes) GO(true); else GO(false);
 #undef GO
     } else {
@@ -859,7 +854,7 @@ int quantize(int64_t rows, int64_t cols, const T* x, int64_t ldx, const T* mask,
         const int per = total >= 16 * 4 * 1024 ? 4 : 1;
         const int64_t wgs = (total + 16 * per - 1) / (16 * per);
         if (wgs > 0xffffff) return fail(NERF_E_ARG, "nerf_fp8_quantize: %lld x %lld is more than one launch covers", (long long)rows, (long long)cols);
-#define GO(N) hipLaunchKernelGGL((k_quantize_rows<T, N>), dim3((unsigned)wgs), dim3(256), 0, stream, rows, cols, x, ldx, wide, (unsigned)blocks, codes, ldc, scales, lds)
+#define GO(N) hipLaunchKernelGGL((k_quantize_rows<T, N>), dim3((unsigned)wgs), dim3(256), 0, stream, rows, cols, x, ldx, (unsigned)blocks, codes, ldc, scales, lds)
         if (per == 4) GO(4); else GO(1);
 #undef GO
     }
@@ -911,8 +906,7 @@ int nerf_fp8_matmul(int64_t m, int64_t n, int64_t k, const uint8_t* a, const uin
     NERF_REQUIRE(((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0 &&
                  ((reinterpret_cast<uintptr_t>(a_scales) | reinterpret_cast<uintptr_t>(b_scales)) & 3) == 0,
                  "nerf_fp8_matmul: codes start at a multiple of 16 bytes, scales of 4");
-    Product p{a, b, a_scales, b_scales, m, n, code_stride(k), scale_stride(k), (int)blocks_of(k), bias, bias_type == NERF_F32, relu, c, ldc,
-              ((reinterpret_cast<uintptr_t>(c) | (uintptr_t)(ldc * elem_size(type))) & 15) == 0};
+    Product p{a, b, a_scales, b_scales, m, n, code_stride(k), scale_stride(k), (int)blocks_of(k), bias, bias_type == NERF_F32, relu, c, ldc};
     hipStream_t stream = as_stream(stream_);
     if (type == NERF_F32) return product<float>(p, k, type, workspace, stream);
     if (type == NERF_BF16) return product<bf16_t>(p, k, type, workspace, stream);

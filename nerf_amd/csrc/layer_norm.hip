@@ -17,9 +17,6 @@ constexpr int LN_SLICES = 1024;         // the most slices of the rows in the we
 constexpr int64_t LN_HELD = 16384;      // rows up to this length are held in registers
 constexpr int LN_GROUPS = 2048;         // the most workgroups of the forward pass
 
-// VEC elements from any element's address (the memory system takes vector accesses at any alignment)
-template <typename T, int VEC>
-struct __attribute__((packed, aligned(sizeof(T)))) Loose { T e[VEC]; };
 template <typename T, int VEC>
 __device__ __forceinline__ Loose<T, VEC> read_raw(const T* row, int i, int c) {      // zeros behind c
     if (i + VEC <= c) return *reinterpret_cast<const Loose<T, VEC>*>(row + i);

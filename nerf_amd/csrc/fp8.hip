@@ -634,63 +634,54 @@ __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, in
     aim(i0, j0);
     clear();
     if constexpr (LONG) {
-        constexpr int X = P + 1, Y = 3, EARLY = M - 1 - X;
-        // The block asked for runs two ahead of the one multiplied, into the next tile where this one ends.  Behind the last it stays
-        // where it is: its rows come once more, for nobody.
-        int ask_tile = blockIdx.x, ask_kb = kb0, ask_words = 0, ask_image = 0;
-        auto ask_next = [&] {
-            ask_image ^= 1;
-            if (ask_kb + 1 < kb1) {
-                ++ask_kb;
-                if ((ask_kb & 3) == 0) ask_words ^= 1;
-            } else if (ask_tile + (int)gridDim.x < total) {
-                ask_tile += gridDim.x;
-                ask_kb = kb0;
-                ask_words ^= 1;
-                int64_t i, j;
-                corner(ask_tile, i, j);
-                aim(i, j);
-            }
+        constexpr int X = P + 1, Y = 3, EARLY = M - X;
+        // The block asked for runs two ahead of the one multiplied: a tile's last two blocks (kb1 >= 2) ask for the next tile's first
+        // two.  Behind the last tile its own first rows come once more, for nobody.  Blocks use the two images in turn, and words of four
+        // blocks' scales the two sets.
+        int image = 0, words = 0;      // words: the set of the tile's first word
+        // block ask_kb is asked for, its scales into the set ask_set; the next block's scales are in next_set, moved by next_shift
+        auto step = [&](int ask_kb, int ask_set, int next_set, int next_shift) {
+            multiply(a0, b0, [&](int i) {
+                if (i < P) fetch(i, image, 1, a1, b1);
+                if (i == X) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // everyone is done with this block's image
+                if (i >= X) issue(i - X, ask_kb, image);
+            });
+            multiply(a1, b1, [&](int i) {
+                if (EARLY + i < N) issue(EARLY + i, ask_kb, image);
+                else if (EARLY + i == N && (ask_kb & 3) == 0) issue_words(ask_kb, ask_set);
+                if (i == Y)      // the next block is in LDS: out are at most the requests made since
+                    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(EARLY + Y + 1) : "memory");
+                if (i > Y && i - Y - 1 < P) fetch(i - Y - 1, image ^ 1, 0, a0, b0);
+                if (i == Y + P + 1) fetch_words(next_set);
+                if (i == M - 1) scales_of(next_shift);
+            });
+            image ^= 1;
         };
-        auto ask_all = [&] {
-            issue_words(ask_kb, ask_words);
+        issue_words(0, 0);
 #pragma unroll
-            for (int i = 0; i < N; ++i) issue(i, ask_kb, ask_image);
-        };
-        ask_all();
-        ask_next();
-        ask_all();
-        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N + WORD_ISSUES) : "memory");
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) issue(i, kb, kb);
+        }
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
 #pragma unroll
         for (int i = 0; i < P; ++i) fetch(i, 0, 0, a0, b0);
         fetch_words(0);
-        int image = 0, set = 0;
+        scales_of(0);
         for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
-            for (int kb = kb0; kb < kb1; ++kb) {
-                ask_next();
-                scales_of(kb);
-                multiply(a0, b0, [&](int i) {
-                    if (i < P) fetch(i, image, 1, a1, b1);
-                    if (i == X) {      // everyone is done with this block's image
-                        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                        issue_words(ask_kb, ask_words);
-                    }
-                    if (i > X) issue(i - X - 1, ask_kb, ask_image);
-                });
-                // (the next block's scales are in the other set where a new word begins: four blocks on, or in another tile)
-                if (kb + 1 == kb1 || ((kb + 1) & 3) == 0) set ^= 1;
-                image ^= 1;
-                multiply(a1, b1, [&](int i) {
-                    if (EARLY + i < N) issue(EARLY + i, ask_kb, ask_image);
-                    if (i == Y)      // the next block is in LDS: out are at most the requests made since
-                        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(WORD_ISSUES + EARLY + Y + 1) : "memory");
-                    if (i > Y && i - Y - 1 < P) fetch(i - Y - 1, image, 0, a0, b0);
-                    if (i == Y + P + 1) fetch_words(set);
-                });
-            }
-            corner(tile, i0, j0);
+            for (int kb = 0; kb < kb1 - 2; ++kb) step(kb + 2, words ^ ((kb + 2) >> 2 & 1), words ^ ((kb + 1) >> 2 & 1), kb + 1);
+            const int next = tile + (int)gridDim.x < total ? tile + (int)gridDim.x : tile;
+            const int next_words = words ^ ((kb1 + 3) >> 2 & 1);
+            int64_t ni, nj;
+            corner(next, ni, nj);
+            aim(ni, nj);
+#pragma unroll 1
+            for (int q = 0; q < 2; ++q) step(q, next_words, q ? next_words : words ^ ((kb1 - 1) >> 2 & 1), q ? 0 : kb1 - 1);
+            words = next_words;
             write(i0, j0);
             clear();
+            i0 = ni;
+            j0 = nj;
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // nothing may arrive in LDS that is another workgroup's by then
     } else {
@@ -789,7 +780,7 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, int type) {
     if ((m <= 64 && few <= many) || k > (1 << 22)) return {0, 1, (int)blocks, 0};
     auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
     const int cus = 256;
-    const int tile = type != NERF_F32 && tiles(256) >= cus ? 256 : 128;
+    const int tile = type != NERF_F32 && blocks > 1 && tiles(256) >= cus ? 256 : 128;      // (large tiles ask for blocks two ahead)
     int64_t slices = 1;
     const int64_t count = tiles(tile);      // (large tiles are never sliced)
     if (count < cus) slices = cus / count;

@@ -10,6 +10,8 @@
 // unscaled fp8 instruction the same), which a 16-bit output, rounded to 2^-9 or 2^-12, does not show.  An fp32 output does: there
 // the codes are decoded to bf16 with their scale (exact: 4 bits into 8, the exponent range is fp32's) and multiplied by the
 // bf16 instruction, whose sums are within 4e-7.
+#include <algorithm>
+#include <cmath>
 #include "common.hpp"
 #include "elem.hpp"
 #include "wave_ops.hpp"
@@ -84,44 +86,35 @@ __device__ __forceinline__ void over_rows(unsigned (&v)[8], unsigned (*red)[QT],
     for (int j = 0; j < 8; ++j) v[j] = op(op(red[0][c + j], red[1][c + j]), op(red[2][c + j], red[3][c + j]));
 }
 
-// Along the columns alone: sixteen lanes hold a block of 128, a workgroup 16 N blocks that follow one another in memory.
-template <typename T, int N>
+// Along the columns alone: sixteen lanes hold a block of 128, a workgroup sixteen blocks that follow one another in memory.  Bounded by
+// memory: 16384 x 4096 bf16 in 34 us, 5.9 TB/s.  (Four blocks a lane were slower at every size: 39 us there, 4 x 8192 3.6 us against 2.0.)
+template <typename T>
 __global__ void __launch_bounds__(256) k_quantize_rows(int64_t rows, int64_t cols, const T* __restrict__ x, int64_t ldx,
                                                        unsigned blocks, uint8_t* __restrict__ codes, int64_t ldc, uint8_t* __restrict__ scales,
                                                        int64_t lds) {
     const int l = threadIdx.x & 15;
-    const int64_t total = rows * blocks, first = (int64_t)blockIdx.x * (16 * N) + (threadIdx.x >> 4);
-    float v[N][8];
-    int64_t row[N];
-    unsigned kb[N];
+    const unsigned id = blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int64_t row = id / blocks;
+    const unsigned kb = id - (unsigned)row * blocks;
+    if (row >= rows) return;
+    const int64_t c = (int64_t)kb * KB + l * 8;
+    float v[8];
+    if (c + 8 <= cols) {
+        load_vec<T, 8>(x + row * ldx + c, v);
+    } else {
 #pragma unroll
-    for (int q = 0; q < N; ++q) {
-        const int64_t id = first + 16 * q;
-        row[q] = total <= 0xffffffffll ? (int64_t)((unsigned)id / blocks) : id / blocks;
-        kb[q] = (unsigned)(id - row[q] * blocks);
-        const int64_t c = (int64_t)kb[q] * KB + l * 8;
-        if (row[q] < rows && c + 8 <= cols) {
-            load_vec<T, 8>(x + row[q] * ldx + c, v[q]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[q][e] = (row[q] < rows && c + e < cols) ? (float)x[row[q] * ldx + c + e] : 0.0f;
-        }
+        for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? (float)x[row * ldx + c + e] : 0.0f;
     }
+    unsigned am = 0;
 #pragma unroll
-    for (int q = 0; q < N; ++q) {
-        unsigned am = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) { const unsigned u = mag_bits(v[q][e]); am = u > am ? u : am; }
-        const int ex = scale_exp(row16_max(am));
-        const float inv = pow2(-ex);
-        if (row[q] >= rows) continue;
-        *reinterpret_cast<uint2*>(codes + row[q] * ldc + (int64_t)kb[q] * KB + l * 8) =
-            make_uint2(pack4(v[q][0], v[q][1], v[q][2], v[q][3], inv), pack4(v[q][4], v[q][5], v[q][6], v[q][7], inv));
-        if (l == 0) {
-            scales[row[q] * lds + kb[q]] = (uint8_t)(ex + 127);
-            if (kb[q] + 1 == blocks)
-                for (int64_t z = blocks; z < lds; ++z) scales[row[q] * lds + z] = 0;
-        }
+    for (int e = 0; e < 8; ++e) { const unsigned u = mag_bits(v[e]); am = u > am ? u : am; }
+    const int ex = scale_exp(row16_max(am));
+    const float inv = pow2(-ex);
+    *reinterpret_cast<uint2*>(codes + row * ldc + c) = make_uint2(pack4(v[0], v[1], v[2], v[3], inv), pack4(v[4], v[5], v[6], v[7], inv));
+    if (l == 0) {
+        scales[row * lds + kb] = (uint8_t)(ex + 127);
+        if (kb + 1 == blocks)
+            for (int64_t z = blocks; z < lds; ++z) scales[row * lds + z] = 0;
     }
 }
 
@@ -780,14 +773,23 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, int type) {
     if ((m <= 64 && few <= many) || k > (1 << 22)) return {0, 1, (int)blocks, 0};
     auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
     const int cus = 256;
-    const int tile = type != NERF_F32 && blocks > 1 && tiles(256) >= cus ? 256 : 128;      // (large tiles ask for blocks two ahead)
-    int64_t slices = 1;
-    const int64_t count = tiles(tile);      // (large tiles are never sliced)
-    if (count < cus) slices = cus / count;
-    if (slices > blocks / 4) slices = blocks / 4;
-    if (slices < 1) slices = 1;
+    const int64_t small = tiles(128);
+    // Large tiles or small: large ones use the matrix instruction better, and a tile costs them more.  What either takes in us, fitted to
+    // 2048 x 2048 to 5632 x 5632 at k = 4096 and 512 and to 65536 x 256 x 256; a round that is not full takes less than a full one.  (16 bits,
+    // large / small: 4096 x 4096 x 4096 62 / 74, 2560 x 3584 x 4096 45 / 55, 5632 x 5632 x 4096 105 / 135, 2048 x 2048 x 4096 61 / 26,
+    // 4096 x 4096 x 512 19.5 / 17.2.)  Large tiles ask for blocks two ahead, so that they need two.
+    const double r = (double)tiles(256) / cus, q = (double)small / (2 * cus);
+    const double large_us = (r + 2 * std::ceil(r)) / 3 * (13.4 + 1.3 * blocks), small_us = (q + std::ceil(q)) / 2 * (4.5 + 1.02 * blocks);
+    if (type != NERF_F32 && blocks > 1 && large_us < small_us) return {256, 1, (int)blocks, cus};
+    // Few small tiles leave compute units idle: k is cut in slices, whose sums a second launch joins.  A block takes 0.76 us, the join
+    // 5 us and what the partial sums cost to write and to read.  (256 x 256 x 65536 fp32: 1 slice 390, 16 slices 34.5, 64 slices 21.0;
+    // 1024 x 1024 x 1024: 1 slice 7.3, 2 slices 12.6.)
+    const int64_t most = small < cus ? std::min(cus / small, blocks) : 1;
+    const double block_us = 0.76, sum_us = 2e-6 * (double)m * n;
+    int64_t slices = std::min(std::max((int64_t)(std::sqrt(blocks * block_us / sum_us) + 0.5), (int64_t)1), most);
+    if (blocks * block_us / slices + 5 + slices * sum_us >= blocks * block_us) slices = 1;
     const int64_t per = (blocks + slices - 1) / slices;
-    return {tile, (int)((blocks + per - 1) / per), (int)per, cus};
+    return {128, (int)((blocks + per - 1) / per), (int)per, cus};
 }
 
 template <typename T>
@@ -840,14 +842,9 @@ int quantize(int64_t rows, int64_t cols, const T* x, int64_t ldx, const T* mask,
         if (codes) GO(true); else GO(false);
 #undef GO
     } else {
-        const int64_t blocks = blocks_of(cols), total = rows * blocks;
-        // four blocks a lane where that still fills the machine, one where latency counts
-        const int per = total >= 16 * 4 * 1024 ? 4 : 1;
-        const int64_t wgs = (total + 16 * per - 1) / (16 * per);
+        const int64_t blocks = blocks_of(cols), wgs = (rows * blocks + 15) / 16;
         if (wgs > 0xffffff) return fail(NERF_E_ARG, "nerf_fp8_quantize: %lld x %lld is more than one launch covers", (long long)rows, (long long)cols);
-#define GO(N) hipLaunchKernelGGL((k_quantize_rows<T, N>), dim3((unsigned)wgs), dim3(256), 0, stream, rows, cols, x, ldx, (unsigned)blocks, codes, ldc, scales, lds)
-        if (per == 4) GO(4); else GO(1);
-#undef GO
+        hipLaunchKernelGGL((k_quantize_rows<T>), dim3((unsigned)wgs), dim3(256), 0, stream, rows, cols, x, ldx, (unsigned)blocks, codes, ldc, scales, lds);
     }
     const int rc = launched("nerf_fp8_quantize");
     if (rc || !col_sum) return rc;

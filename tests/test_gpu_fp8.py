@@ -141,16 +141,16 @@ def test_products(device, m, n, k, out):
     assert torch.equal(ops.matmul_fp8(a, b, out_dtype=out), ops.matmul_fp8(a, b, out_dtype=out))
 
 
-@pytest.mark.parametrize("m,n,k", [(4353, 4360, 100), (4352, 4609, 300), (4608, 4352, 1100)])
+@pytest.mark.parametrize("m,n,k", [(4353, 4360, 100), (4096, 8192, 768), (4090, 8187, 1000), (6100, 8190, 700)])
 @pytest.mark.parametrize("out", TYPES[1:], ids=IDS[1:])
 def test_more_large_tiles_than_workgroups(device, m, n, k, out):
-    """A workgroup takes several tiles, and asks for the next one's rows while it finishes the last: one, three and nine blocks of k."""
+    """Large tiles, of which a workgroup takes two or three, asking for the next one's rows while it finishes the last; and small ones."""
     from nerf_amd import ops
     a, b = ops.quantize_fp8(_data(m, k, torch.float32, device, m)), ops.quantize_fp8(_data(n, k, torch.float32, device, n + 1))
     bias = _data(1, n, out, device, 7)[0]
     got = ops.matmul_fp8(a, b, bias, out_dtype=out)
-    va, vb = _values(a)[0], _values(b)[0]
-    want, mag = va @ vb.t() + bias.cpu().double(), va.abs() @ vb.abs().t() + bias.cpu().double().abs()
+    va, vb, vbias = _values(a)[0].to(device), _values(b)[0].to(device), bias.double()
+    want, mag = (va @ vb.t() + vbias).cpu(), (va.abs() @ vb.abs().t() + vbias.abs()).cpu()
     _check(got, want, mag, k, (m, n, k, out))
     assert torch.equal(ops.matmul_fp8(a, b, bias, out_dtype=out), got)
 

@@ -12,8 +12,7 @@
 // same bits.  A positive v never becomes 0, because it divides.
 //
 // Bounded by memory: 235.8 M bf16 parameters with their master copies (30 bytes each) in 1.30 ms, 5.4 TB/s; 59.1 M fp32 with states in 8 bits
-// (16.1 bytes) in 173-185 us, 5.1-5.5 TB/s; 48 tensors of a small network's in 7 us, behind the 3 us of the coefficients.  A launch for each
-// tensor would cost 48 times that.
+// (16.1 bytes) in 173-185 us, 5.1-5.5 TB/s; the 48 tensors of a small pair of networks in 7 us, behind the 3 us of the coefficients.
 #include "common.hpp"
 #include "elem.hpp"
 

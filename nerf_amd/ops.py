@@ -1078,7 +1078,7 @@ def _quantize(x: torch.Tensor, want: bool, want_t: bool, mask: Optional[torch.Te
 def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
     """x [rows, k] (fp32, bf16 or fp16) in e4m3 with one power-of-two scale per row and 128 values of k: the smallest that takes
     the block's largest value to at most 448, so that every value is rounded (to nearest even) once.  A value that is not finite
-    becomes NaN."""
+    becomes NaN.  What comes out is not part of x's graph (linear_fp8 quantises inside and is)."""
     if x.dim() != 2:
         raise ValueError(f"quantize_fp8: expected a matrix, got shape {tuple(x.shape)}")
     return _quantize(x.detach(), True, False)[0]
@@ -1086,7 +1086,9 @@ def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
 
 def matmul_fp8(a: Fp8Rows, b: Fp8Rows, bias: Optional[torch.Tensor] = None, relu: bool = False,
                out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """a [m, k] b [n, k]^T + bias [n] (+ ReLU) in out_dtype (fp32, bf16 or fp16); sums in fp32."""
+    """a [m, k] b [n, k]^T + bias [n] (+ ReLU) in out_dtype (fp32, bf16 or fp16); sums in fp32.  No backward pass."""
+    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
+        raise ValueError("matmul_fp8: no backward pass for the bias; call it under torch.no_grad()")
     if not (isinstance(a, Fp8Rows) and isinstance(b, Fp8Rows)):
         raise TypeError("matmul_fp8: expected two Fp8Rows")
     if a.k != b.k:

@@ -381,6 +381,11 @@ class AdamW(torch.optim.Optimizer):
             plan = self._plans.get(id(group)) if known else None
             if plan is None or not plan.stands(group["params"], grads):
                 plan = self._plans[id(group)] = _Plan(self, group["params"], grads)
+            lr = group["lr"]
+            if torch.is_tensor(lr) and lr.is_cuda:
+                for launch in plan.launches:
+                    if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != launch.device:
+                        raise TypeError(f"AdamW: a device learning rate must be one fp32 value on {launch.device}, got {lr.dtype} on {lr.device}")
             work += [(group, launch, launch.take(grads)) for launch in plan.launches]
         self._seen = list(self.state.values())
         for group, launch, (addresses, _) in work:
@@ -390,8 +395,6 @@ class AdamW(torch.optim.Optimizer):
     def _launch(self, group, launch, grads):
         device, lr, lr_dev = launch.device, group["lr"], None
         if torch.is_tensor(lr) and lr.is_cuda:
-            if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != device:
-                raise TypeError(f"AdamW: a device learning rate must be one fp32 value on {device}, got {lr.dtype} on {lr.device}")
             lr_dev, lr = lr.data_ptr(), 0.0
         n = len(launch.params)
         coef = torch.empty((4 * n,), dtype=torch.float32, device=device)
@@ -404,8 +407,12 @@ class AdamW(torch.optim.Optimizer):
 
     # ---- checkpoints ---------------------------------------------------------------------------------
     def load_state_dict(self, state_dict):
-        """Checkpoints of this class with the same state_bits, and of torch.optim.Adam / AdamW with state_bits = 32.  The states keep
-        their own types (torch.optim would cast them to the parameter's)."""
+        """Checkpoints of this class with the same state_bits, and of torch.optim.Adam / AdamW with state_bits = 32, where their rule is this
+        one's: no amsgrad, no maximize, no weight decay in Adam's gradient.  The states keep their own types (torch.optim would cast them
+        to the parameter's)."""
+        for g in state_dict["param_groups"]:
+            if g.get("amsgrad") or g.get("maximize") or (g.get("weight_decay") and g.get("decoupled_weight_decay") is False):
+                raise ValueError("AdamW: a checkpoint with amsgrad, maximize or a weight decay that is part of the gradient")
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         fresh = {}

@@ -421,6 +421,13 @@ def test_refusals(device):
     t.grad = torch.zeros(8, 6, device=device)
     with pytest.raises(ValueError, match="contiguous"):
         AdamW([t]).step()
+    # nothing is launched when a later group cannot be: neither its parameters nor an earlier group's move
+    a, b = _params([(5,), (6,)], torch.float32, device, 12)
+    two = AdamW([{"params": [a]}, {"params": [b], "lr": torch.tensor(1e-3, dtype=torch.float64, device=device)}])
+    before = a.detach().clone()
+    with pytest.raises(TypeError, match="learning rate"):
+        two.step()
+    assert torch.equal(a, before) and float(two.state[a]["step"]) == 0.0
     # a gradient of another layout is copied, not refused
     q = torch.nn.Parameter(torch.zeros(8, 6, device=device))
     q.grad = torch.arange(48.0, device=device).view(6, 8).t()

@@ -85,6 +85,8 @@ def test_quantisation_is_the_definition(device, r, k, dtype):
     wide[:, 3:] = x
     assert torch.equal(_values(ops.quantize_fp8(wide[:, 3:]))[0], want)
     assert torch.equal(_values(ops.quantize_fp8(x.t().contiguous().t()))[0], want)
+    for got in ops._quantize(wide[:, 3:], True, True)[:2]:
+        assert torch.equal(_values(got)[0], want if got.k == k and got.rows == r else _oracle_quantize(x.double().cpu().t())[0])
     # both directions and the column sums at once, with a mask
     mask = torch.randn(r, k, device=device).to(dtype)
     mask[0, 0] = float("nan")
@@ -232,6 +234,18 @@ def test_shapes_broadcasts_and_empty_batches(device):
     assert e.grad.shape == (0, 50) and not w.grad.any() and not b.grad.any()
     v = torch.randn(50, device=device)
     assert torch.equal(ops.linear_fp8(v, w.detach()), ops.linear_fp8(v[None], w.detach())[0])
+
+
+def test_no_gradient_is_lost_silently(device):
+    from nerf_amd import ops
+    a, b = ops.quantize_fp8(torch.randn(4, 70, device=device)), ops.quantize_fp8(torch.randn(6, 70, device=device))
+    bias = torch.zeros(6, device=device, requires_grad=True)
+    with pytest.raises(ValueError, match="no backward pass"):
+        ops.matmul_fp8(a, b, bias)
+    with pytest.raises(ValueError, match="no backward pass"):
+        ops.linear_fp8(torch.randn(4, 70, device=device), b, bias)
+    with torch.no_grad():
+        assert ops.matmul_fp8(a, b, bias).shape == (4, 6)
 
 
 def test_streams_and_graphs(device):

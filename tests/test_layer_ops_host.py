@@ -95,6 +95,12 @@ def test_adamw_argument_errors():
         opt.step()
     assert not opt.state
     assert opt.param_groups[0]["capturable"]
+    # rules that are not this one's are refused, whole, before anything is taken over
+    for stock in (torch.optim.AdamW([p], amsgrad=True), torch.optim.AdamW([p], maximize=True), torch.optim.Adam([p], weight_decay=0.1)):
+        with pytest.raises(ValueError, match="amsgrad, maximize"):
+            opt.load_state_dict(stock.state_dict())
+    opt.load_state_dict(torch.optim.Adam([p], lr=0.25).state_dict())
+    assert opt.param_groups[0]["lr"] == 0.25 and opt.param_groups[0]["capturable"]
 
 
 def test_options_of_the_training_command():

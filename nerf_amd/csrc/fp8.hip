@@ -500,7 +500,7 @@ struct TileLds {      // two images, two sets of scale words, a band of eight ro
 // block they were half of them (8192 x 8192 x 16384: 848 -> 746 us).
 // 256 x 256, bf16 of random codes: 8192^3 in 385 us (2.86 PFLOP/s), 16384 x 8192 x 4096 in 418 us (2.63); of zeros 277 us -- the board's power
 // limit takes the rest, the matrix pipe is busy 81 % of the cycles, 15 % are waits at the two barriers of a block.  128 x 128, fp32: 8192^3
-// in 880 us (1.25 PFLOP/s, the bf16 instruction's), 65536 x 256 x 256 in 18 us (4.7 TB/s).
+// in 845 us (1.30 PFLOP/s, of the bf16 instruction), 65536 x 256 x 256 in 18-20 us (4.2-4.7 TB/s).
 template <typename T, int BM, int BN>
 __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, int tiles_n, int blocks_per_slice, float* __restrict__ partial) {
     constexpr bool F32 = sizeof(T) == 4;
@@ -707,7 +707,7 @@ __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, in
             __builtin_amdgcn_sched_barrier(0);
             multiply(a1, b1, [&](int i) {
                 if constexpr (decltype(more)::value) {
-                    if (i == 0) issue_words(kb + 2, place_of(kb + 2));
+                    if (i == 0 && ((kb + 2) & 3) == 0) issue_words(kb + 2, place_of(kb + 2));
 #pragma unroll
                     for (int q = i * N / M; q < (i + 1) * N / M; ++q) issue(q, kb + 2, kb & 1);
                 }

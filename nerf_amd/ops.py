@@ -6,6 +6,7 @@ if the library reports an error.
 """
 from __future__ import annotations
 
+import functools
 import os
 from typing import Optional, Sequence
 
@@ -909,6 +910,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], 
 # ------------------------------------------------------------------------------------------------
 # layers of wide networks: layer norm, products in 8 bits
 # ------------------------------------------------------------------------------------------------
+_empty_like, _CONTIGUOUS = torch.empty_like, torch.contiguous_format
+# (the library's size queries depend on their arguments alone; a call through ctypes costs more than looking its answer up)
+_layer_norm_workspace, _matmul_workspace, _linear_kept, _linear_workspace = (
+    functools.lru_cache(maxsize=1024)(f) for f in (lib.nerf_layer_norm_workspace_floats, lib.nerf_fp8_matmul_workspace_floats,
+                                                   lib.nerf_linear_fp8_kept_bytes, lib.nerf_linear_fp8_workspace_bytes))
 ELEM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # NERF_F32, NERF_BF16, NERF_F16
 
 
@@ -980,14 +986,14 @@ def _layer_norm_forward(x: torch.Tensor, w, b, eps: float, need_grad: bool):
     w_dtype = dtype if wc is None and bc is None else (bc if wc is None else wc).dtype
     if wc is not None and bc is not None and bc.dtype != w_dtype:
         raise TypeError(f"layer_norm: weight is {wc.dtype}, bias {bc.dtype}")
-    y = torch.empty(x.shape, dtype=dtype, device=dev)
+    y = _empty_like(x, memory_format=_CONTIGUOUS)
     stats = torch.empty((3, n), dtype=torch.float32, device=dev) if need_grad else None
     kind, w_kind = ELEM_TYPES[dtype], ELEM_TYPES[w_dtype]
     _launch(dev, "layer_norm", 2 * n * c * dtype.itemsize, lib.nerf_layer_norm_fwd, n, c, kind, x2.data_ptr(), ld, w_kind, _ptr(wc), _ptr(bc), eps,
             y.data_ptr(), c, _ptr(stats))
     if not need_grad:
         return y, None
-    return y, ((x2, wc, stats), (n, c, ld, kind, w_kind, dtype, w_dtype, dev, lib.nerf_layer_norm_workspace_floats(n, c)))
+    return y, ((x2, wc, stats), (n, c, ld, kind, w_kind, w_dtype, dev, _layer_norm_workspace(n, c)))
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -1003,14 +1009,20 @@ class _LayerNorm(torch.autograd.Function):
     @_differentiable_once
     def backward(ctx, dy):
         x2, wc, stats = ctx.saved_tensors
-        n, c, ld, kind, w_kind, dtype, w_dtype, dev, floats = ctx.args
-        dy2, _, ld_dy = _rows_any(dy, "grad")
+        n, c, ld, kind, w_kind, w_dtype, dev, floats = ctx.args
+        dy2, ld_dy = dy, c
+        if not dy.is_contiguous():
+            dy2, _, ld_dy = _rows_any(dy, "grad")
         need_dx, need_dw, need_db, _ = ctx.needs_input_grad
-        dx = torch.empty(dy.shape, dtype=dtype, device=dev) if need_dx else None
-        dw = torch.empty((c,), dtype=w_dtype, device=dev) if need_dw else None
-        db = torch.empty((c,), dtype=w_dtype, device=dev) if need_db else None
-        ws = torch.empty((floats,), dtype=torch.float32, device=dev) if need_dw or need_db else None
-        _launch(dev, "layer_norm_bwd", 3 * n * c * dtype.itemsize, lib.nerf_layer_norm_bwd, n, c, kind, x2.data_ptr(), ld, dy2.data_ptr(), ld_dy,
+        dx = _empty_like(dy, memory_format=_CONTIGUOUS) if need_dx else None
+        dw = db = ws = None
+        if need_dw or need_db:
+            ws = stats.new_empty(floats)
+            if need_dw:
+                dw = _empty_like(wc)
+            if need_db:
+                db = torch.empty((c,), dtype=w_dtype, device=dev) if wc is None else _empty_like(wc)
+        _launch(dev, "layer_norm_bwd", 3 * n * c * dy.itemsize, lib.nerf_layer_norm_bwd, n, c, kind, x2.data_ptr(), ld, dy2.data_ptr(), ld_dy,
                 w_kind, _ptr(wc), stats.data_ptr(), _ptr(dx), c, _ptr(dw), _ptr(db), _ptr(ws))
         return dx, dw, db, None
 
@@ -1101,7 +1113,7 @@ def matmul_fp8(a: Fp8Rows, b: Fp8Rows, bias: Optional[torch.Tensor] = None, relu
     c = torch.empty((a.rows, b.rows), dtype=out_dtype, device=dev)
     bias = _vector(bias, b.rows, c, "bias")
     kind = ELEM_TYPES[out_dtype]
-    floats = lib.nerf_fp8_matmul_workspace_floats(a.rows, b.rows, a.k, kind)
+    floats = _matmul_workspace(a.rows, b.rows, a.k, kind)
     ws = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
     _launch(dev, "fp8_matmul", 2 * a.rows * b.rows * a.k, lib.nerf_fp8_matmul, a.rows, b.rows, a.k, a.codes.data_ptr(), a.scales.data_ptr(),
             b.codes.data_ptr(), b.scales.data_ptr(), kind if bias is None else ELEM_TYPES[bias.dtype], _ptr(bias), int(bool(relu)), kind,
@@ -1124,8 +1136,8 @@ def _linear_fp8_forward(x: torch.Tensor, weight, b, relu: bool, need_dx: bool, n
         w_args = (ELEM_TYPES[w2.dtype], w2.data_ptr(), ldw, None, None)
     bias = _vector(b, n_out, x2, "bias")
     y = torch.empty(x.shape[:-1] + (n_out,), dtype=x2.dtype, device=dev)
-    kept = _bytes(lib.nerf_linear_fp8_kept_bytes(n, n_in, n_out, need_dx, need_dw), dev) if need_dx or need_dw else None
-    ws = _bytes(lib.nerf_linear_fp8_workspace_bytes(n, n_in, n_out, kind, 0, 0), dev)
+    kept = _bytes(_linear_kept(n, n_in, n_out, need_dx, need_dw), dev) if need_dx or need_dw else None
+    ws = _bytes(_linear_workspace(n, n_in, n_out, kind, 0, 0), dev)
     _launch(dev, "linear_fp8", 2 * n * n_in * n_out, lib.nerf_linear_fp8_fwd, n, n_in, n_out, kind, x2.data_ptr(), ld, *w_args,
             kind if bias is None else ELEM_TYPES[bias.dtype], _ptr(bias), int(relu), y.data_ptr(), _ptr(kept), need_dx, need_dw, _ptr(ws))
     return y, kept, (n, n_in, n_out, kind, dev)
@@ -1142,22 +1154,24 @@ class _LinearFp8(torch.autograd.Function):
         ctx.save_for_backward(kept, y if relu else None)
         n, n_in, n_out, kind, _ = sizes
         w_kind = ELEM_TYPES[w.dtype]
-        ctx.args = sizes + (need_dx, need_dw, x.dtype, w.dtype, w_kind, None if b is None else b.dtype,
-                            lib.nerf_linear_fp8_workspace_bytes(n, n_in, n_out, kind, w_kind, 1))
+        ctx.args = sizes + (need_dx, need_dw, w.dtype, w_kind, None if b is None else b.dtype,
+                            _linear_workspace(n, n_in, n_out, kind, w_kind, 1))
         return y
 
     @staticmethod
     @_differentiable_once
     def backward(ctx, dy):
         kept, y = ctx.saved_tensors
-        n, n_in, n_out, kind, dev, kept_dx, kept_dw, dtype, w_dtype, w_kind, b_dtype, count = ctx.args
+        n, n_in, n_out, kind, dev, kept_dx, kept_dw, w_dtype, w_kind, b_dtype, count = ctx.args
         need_dx, need_dw, need_db, _ = ctx.needs_input_grad
-        dx = torch.empty(dy.shape[:-1] + (n_in,), dtype=dtype, device=dev) if need_dx else None
+        dx = dy.new_empty(dy.shape[:-1] + (n_in,)) if need_dx else None
         if n == 0:
             dw = torch.zeros((n_out, n_in), dtype=w_dtype, device=dev) if need_dw else None
             db = torch.zeros((n_out,), dtype=b_dtype, device=dev) if need_db else None
             return dx, dw, db, None
-        dy2, _, ld = _rows_any(dy, "grad")
+        dy2, ld = dy, n_out
+        if not dy.is_contiguous():
+            dy2, _, ld = _rows_any(dy, "grad")
         dw = torch.empty((n_out, n_in), dtype=w_dtype, device=dev) if need_dw else None
         db = torch.empty((n_out,), dtype=b_dtype, device=dev) if need_db else None
         ws = torch.empty((count,), dtype=torch.uint8, device=dev)

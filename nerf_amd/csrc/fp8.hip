@@ -45,29 +45,50 @@ __device__ __forceinline__ unsigned row16_max(unsigned v) {
     return max_ror<0x128>(v);
 }
 
-// bits of |v| for the largest of a block; what is not finite has no part in it
-__device__ __forceinline__ unsigned mag_bits(float v) {
-    const unsigned u = __float_as_uint(v) & 0x7fffffffu;
-    return u < 0x7f800000u ? u : 0u;
-}
+__device__ __forceinline__ unsigned mag_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+constexpr unsigned INF_BITS = 0x7f800000u;
+
 // smallest e >= -126 with amax <= 448 * 2^e, from amax's bits (448 = 1.75 * 2^8)
 __device__ __forceinline__ int scale_exp(unsigned amax) {
     const int e = (int)(amax >> 23) - 127 - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
     return e < -126 ? -126 : e;
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }      // -126 <= e <= 127
-// x * inv in e4m3, four to a word; what is not finite becomes NaN
-__device__ __forceinline__ float finite_or_nan(float v) {
-    return (__float_as_uint(v) & 0x7fffffffu) < 0x7f800000u ? v : __uint_as_float(0x7fc00000u);
-}
+// x * inv in e4m3, four to a word
 __device__ __forceinline__ unsigned pack4(float a, float b, float c, float d, float inv) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(finite_or_nan(a) * inv, finite_or_nan(b) * inv, 0, false);
-    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(finite_or_nan(c) * inv, finite_or_nan(d) * inv, w, true);
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, w, true);
+}
+// What is not finite has no part in its block's largest value and becomes NaN.  A wave that meets such values (seen from its largest bits)
+// takes them out, as zeros, remembers where they were, and puts the NaNs into the codes; the other waves pay for nothing.
+template <int R>
+__device__ __forceinline__ unsigned take_out(float (&v)[R][8]) {      // bit 8 q + e
+    unsigned where = 0;
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool bad = mag_bits(v[q][e]) >= INF_BITS;
+            where |= (bad ? 1u : 0u) << (8 * q + e);
+            v[q][e] = bad ? 0.0f : v[q][e];
+        }
+    return where;
+}
+__device__ __forceinline__ unsigned nan_bytes(unsigned where, int first, int step) {      // NaN codes of four of the places
+    unsigned w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= (where >> (first + i * step) & 1u) * (0x7fu << (8 * i));
+    return w;
+}
+__device__ __forceinline__ unsigned largest(const float (&v)[8]) {
+    unsigned am = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { const unsigned u = mag_bits(v[e]); am = u > am ? u : am; }
+    return am;
 }
 
 constexpr int QT = 128;       // a workgroup quantises a tile of 128 x 128
 constexpr int QLD = QT + 16;
-
 constexpr int QR = 4, Q_THREADS = QT / QR * (QT / 8), Q_WAVES = Q_THREADS / 64;      // a thread's rows, of eight columns
 
 // eight columns' values over a wave's four threads of each, to red[wave]
@@ -97,19 +118,22 @@ __global__ void __launch_bounds__(256) k_quantize_rows(int64_t rows, int64_t col
     const unsigned kb = id - (unsigned)row * blocks;
     if (row >= rows) return;
     const int64_t c = (int64_t)kb * KB + l * 8;
-    float v[8];
+    float v[1][8];
     if (c + 8 <= cols) {
-        load_vec<T, 8>(x + row * ldx + c, v);
+        load_vec<T, 8>(x + row * ldx + c, v[0]);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? (float)x[row * ldx + c + e] : 0.0f;
+        for (int e = 0; e < 8; ++e) v[0][e] = c + e < cols ? (float)x[row * ldx + c + e] : 0.0f;
     }
-    unsigned am = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) { const unsigned u = mag_bits(v[e]); am = u > am ? u : am; }
+    unsigned am = largest(v[0]), where = 0;
+    if (__any(am >= INF_BITS)) {
+        where = take_out(v);
+        am = largest(v[0]);
+    }
     const int ex = scale_exp(row16_max(am));
     const float inv = pow2(-ex);
-    *reinterpret_cast<uint2*>(codes + row * ldc + c) = make_uint2(pack4(v[0], v[1], v[2], v[3], inv), pack4(v[4], v[5], v[6], v[7], inv));
+    *reinterpret_cast<uint2*>(codes + row * ldc + c) = make_uint2(pack4(v[0][0], v[0][1], v[0][2], v[0][3], inv) | nan_bytes(where, 0, 1),
+                                                                  pack4(v[0][4], v[0][5], v[0][6], v[0][7], inv) | nan_bytes(where, 4, 1));
     if (l == 0) {
         scales[row * lds + kb] = (uint8_t)(ex + 127);
         if (kb + 1 == blocks)
@@ -120,8 +144,8 @@ __global__ void __launch_bounds__(256) k_quantize_rows(int64_t rows, int64_t col
 // codes / scales: along the columns (rows keep their order); codes_t / scales_t: of the transpose, along the rows; colsum: sums of the
 // tile's columns, [tile row][cols].  mask: values whose mask entry is <= 0 count as 0 (the gradient of a ReLU's output).
 // One pass over x whatever is asked for; the transposed codes are packed along the rows in registers and cross the workgroup as bytes.
-// Bounded by memory where there is enough of it: both codes of 16384 x 4096 bf16 in 60 us, 4.5 TB/s; of 1001 x 333 in 9.4 us, most of it
-// one pass through the instructions.  (Eight rows a thread: 70 us and 14 us.)
+// Bounded by memory where there is enough of it: both codes of 16384 x 4096 bf16 in 49 us, 5.5 TB/s; of 1001 x 333 in 9 us, most of it
+// one pass through the instructions.  (Eight rows a thread: 70 us and 14 us; with every value looked at for being finite 61 us.)
 template <typename T, bool ROWS>
 __global__ void __launch_bounds__(Q_THREADS, 4) k_quantize(int64_t rows, int64_t cols, unsigned col_tiles, const T* __restrict__ x, int64_t ldx,
                                                   const T* __restrict__ mask, int64_t ldm, uint8_t* __restrict__ codes, int64_t ldc,
@@ -159,26 +183,6 @@ __global__ void __launch_bounds__(Q_THREADS, 4) k_quantize(int64_t rows, int64_t
             for (int e = 0; e < 8; ++e) v[q][e] = m[e] <= 0.0f ? 0.0f : v[q][e];
         }
     }
-    if (ROWS) {
-#pragma unroll
-        for (int q = 0; q < QR; ++q) {
-            const int64_t r = r0 + rl + q;
-            unsigned am = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) { const unsigned u = mag_bits(v[q][e]); am = u > am ? u : am; }
-            const int ex = scale_exp(row16_max(am));
-            const float inv = pow2(-ex);
-            if (r < rows) {
-                const uint2 w = make_uint2(pack4(v[q][0], v[q][1], v[q][2], v[q][3], inv), pack4(v[q][4], v[q][5], v[q][6], v[q][7], inv));
-                *reinterpret_cast<uint2*>(codes + r * ldc + c) = w;
-                if ((tid & 15) == 0) {
-                    scales[r * lds + col_tile] = (uint8_t)(ex + 127);
-                    if (col_tile + 1 == col_tiles)
-                        for (int64_t z = col_tiles; z < lds; ++z) scales[r * lds + z] = 0;
-                }
-            }
-        }
-    }
     // the columns: sums and largest values of the waves' rows, then one thread for each column
     __shared__ unsigned red[2][Q_WAVES][QT];
     __shared__ __attribute__((aligned(16))) float unit[QT];      // 2^-e of the columns
@@ -192,6 +196,39 @@ __global__ void __launch_bounds__(Q_THREADS, 4) k_quantize(int64_t rows, int64_t
             sum[j] = __float_as_uint(t);
         }
         over_rows(sum, red[0], [](unsigned a, unsigned b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); });
+    }
+    unsigned row_am[QR], where = 0, top = 0;
+#pragma unroll
+    for (int q = 0; q < QR; ++q) {
+        row_am[q] = largest(v[q]);
+        top = row_am[q] > top ? row_am[q] : top;
+    }
+    const bool some_bad = __any(top >= INF_BITS);
+    if (some_bad) {
+        where = take_out(v);
+#pragma unroll
+        for (int q = 0; q < QR; ++q) row_am[q] = largest(v[q]);
+    }
+    if (ROWS) {
+#pragma unroll
+        for (int q = 0; q < QR; ++q) {
+            const int64_t r = r0 + rl + q;
+            const int ex = scale_exp(row16_max(row_am[q]));
+            const float inv = pow2(-ex);
+            if (r < rows) {
+                uint2 w = make_uint2(pack4(v[q][0], v[q][1], v[q][2], v[q][3], inv), pack4(v[q][4], v[q][5], v[q][6], v[q][7], inv));
+                if (some_bad) {
+                    w.x |= nan_bytes(where, 8 * q, 1);
+                    w.y |= nan_bytes(where, 8 * q + 4, 1);
+                }
+                *reinterpret_cast<uint2*>(codes + r * ldc + c) = w;
+                if ((tid & 15) == 0) {
+                    scales[r * lds + col_tile] = (uint8_t)(ex + 127);
+                    if (col_tile + 1 == col_tiles)
+                        for (int64_t z = col_tiles; z < lds; ++z) scales[r * lds + z] = 0;
+                }
+            }
+        }
     }
     if (codes_t) {
         unsigned am[8];
@@ -231,13 +268,16 @@ __global__ void __launch_bounds__(Q_THREADS, 4) k_quantize(int64_t rows, int64_t
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const float inv = unit[cl + j];
-        *reinterpret_cast<unsigned*>(bytes + (cl + j) * QLD + rl) = pack4(v[0][j], v[1][j], v[2][j], v[3][j], inv);
+        unsigned w = pack4(v[0][j], v[1][j], v[2][j], v[3][j], inv);
+        if (some_bad) w |= nan_bytes(where, j, 8);
+        // (sixteen bytes of a column lie at their place ^ (column / 16): the lanes of a wave write to all banks)
+        *reinterpret_cast<unsigned*>(bytes + (cl + j) * QLD + (rl ^ ((cl >> 4) << 4))) = w;
     }
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < QT * QT / 16 / Q_THREADS; ++q) {
         const int piece = tid + Q_THREADS * q, col = piece >> 3, k = (piece & 7) * 16;
-        if (c0 + col < cols) *reinterpret_cast<uint4*>(codes_t + (c0 + col) * ldct + r0 + k) = *reinterpret_cast<const uint4*>(bytes + col * QLD + k);
+        if (c0 + col < cols) *reinterpret_cast<uint4*>(codes_t + (c0 + col) * ldct + r0 + k) = *reinterpret_cast<const uint4*>(bytes + col * QLD + (k ^ ((col >> 4) << 4)));
     }
 }
 

@@ -117,6 +117,26 @@ def test_extreme_values(device):
     assert bool(relu[:2].isnan().all()) and bool((relu[2] >= 0).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_values_that_are_not_finite_stay_in_their_place(device, dtype):
+    """In both directions at once: NaN codes exactly there, everyone else's code and scale as if they were not there."""
+    from nerf_amd import ops
+    x = _data(300, 290, torch.float32, device, 5).to(dtype)
+    for i, j, v in ((0, 0, "inf"), (5, 130, "nan"), (6, 131, "-inf"), (127, 127, "nan"), (128, 128, "inf"), (299, 289, "nan"), (40, 200, "-inf")):
+        x[i, j] = float(v)
+    x[200:, 250] = float("nan")          # a whole column of a tile
+    x[257, :] = float("inf")             # whole blocks of a row
+    q, qt, s = ops._quantize(x, True, True, None, torch.float32)
+    wide = x.double().cpu()
+    for got, w in ((q, wide), (qt, wide.t())):
+        want, e = _oracle_quantize(w)
+        v, ge = _values(got)
+        assert _same(v, want) and torch.equal(ge, e.int())
+    bad = ~wide.isfinite().all(0)
+    assert bool((~s.isfinite().cpu() == bad).all())
+    assert _same(_values(ops.quantize_fp8(x))[0], _oracle_quantize(wide)[0])
+
+
 PRODUCTS = [(1, 1, 1), (1, 17, 128), (4, 300, 1000), (16, 16, 128), (17, 33, 129), (64, 256, 256), (65, 100, 384), (100, 64, 77), (129, 130, 257),
             (256, 256, 1024), (300, 520, 640), (1, 4096, 2048), (33, 31, 8192), (1000, 4, 256), (513, 700, 90), (260, 1030, 2100), (40, 24, 20000)]
 

@@ -216,6 +216,19 @@ def test_linear_and_its_gradients(device, n, k, m, relu, dtype, w_dtype):
         assert torch.equal(ops.linear_fp8(x, held, b, relu), y)
 
 
+def test_more_rows_than_a_tile_product_takes_along_k(device):
+    """The weight's gradient over 2^22 + 300 rows: its k is more than the tiles' offsets reach."""
+    from nerf_amd import ops
+    n, k, m = 2 ** 22 + 300, 24, 20
+    x, w = torch.randn(n, k, device=device), torch.randn(m, k, device=device, requires_grad=True)
+    dy = torch.randn(n, m, device=device)
+    y = ops.linear_fp8(x, w)
+    (dw,) = torch.autograd.grad(y, w, dy)
+    xt, gt = ops._quantize(x, False, True)[1], ops._quantize(dy, False, True)[1]
+    vx, vg = _values(xt)[0].to(device), _values(gt)[0].to(device)
+    _check(dw, (vg @ vx.t()).cpu(), (vg.abs() @ vx.abs().t()).cpu(), n, "dw")
+
+
 def test_gradients_against_differences_where_eight_bits_are_exact(device):
     """Small whole numbers are their own e4m3 codes, so the product is the plain one and its differences are the gradient."""
     from nerf_amd import ops

@@ -69,7 +69,7 @@ struct Param {
 };
 
 template <int CTRL>
-__device__ __forceinline__ float add_ror(float v) {
+__device__ __forceinline__ float add_from(float v) {
     return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
 }
 
@@ -91,10 +91,12 @@ __device__ __forceinline__ void row_sum(float (&v)[K], float* part) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         if constexpr (S::L == 16) {
-            v[k] = add_ror<0x121>(v[k]);      // row_ror:1, 2, 4, 8
-            v[k] = add_ror<0x122>(v[k]);
-            v[k] = add_ror<0x124>(v[k]);
-            v[k] = add_ror<0x128>(v[k]);
+            // (pairs that exchange: both lanes add the same two values, so that all sixteen end with the same bits; a mean that differed
+            // from lane to lane would not be the one that the second pass corrects)
+            v[k] = add_from<0xB1>(v[k]);       // quad_perm 1 0 3 2
+            v[k] = add_from<0x4E>(v[k]);       // quad_perm 2 3 0 1
+            v[k] = add_from<0x141>(v[k]);      // row_half_mirror
+            v[k] = add_from<0x140>(v[k]);      // row_mirror
         } else {
             v[k] = wave_sum_f32(v[k]);
         }

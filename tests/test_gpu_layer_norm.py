@@ -109,7 +109,7 @@ def test_row_strides_and_missing_parameters(device, n, c, pad, dtype):
 def test_large_offsets_keep_their_precision(device):
     """Rows whose offset is 1000 times their spread: the values are exact, so the definition's bound holds as anywhere else."""
     from nerf_amd import ops
-    for c in (100, 1024, 5000, 40000):
+    for c in (40, 64, 100, 200, 1024, 1500, 5000, 40000):
         x, w, b, dy = _data(6, c, torch.float32, device, c, offset=1500.0)
         xl = x.requires_grad_(True)
         y = ops.layer_norm(xl, w, b)

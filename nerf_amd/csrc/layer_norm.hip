@@ -4,6 +4,7 @@
 // All sums in fp32.  The mean is kept as a pair: mu1, the rounded sum over C, and mu2, the mean of x - mu1 -- the second pass
 // over the row sums the differences for the variance anyway, and with mu2 a row whose offset is large against its spread loses
 // nothing (a mean rounded to fp32 alone shifts every xh by up to 2^-24 |mu| / sigma).
+#include <algorithm>
 #include <type_traits>
 #include "common.hpp"
 #include "elem.hpp"
@@ -401,14 +402,24 @@ __global__ void __launch_bounds__(LF_COLS * LF_ROWS) k_ln_finish(int slices, int
     }
 }
 
-// The shape that holds rows of c elements: the fewest lanes at first (short rows: several to a wave), then more elements a lane, then
-// more waves: 16 elements a lane of x, dy, the weight, both sums and the next row are what leaves four waves to a SIMD.  (Rows of 1025 to
-// 2048 on two waves instead of four: forward 32 -> 24 us, 16384 x 1100 bf16; backward 43 -> 49 us.)
-template <bool FORWARD, typename F>
+// The shape that holds rows of c elements of `size` bytes: the fewest lanes at first (short rows: several to a wave, 16 bytes a lane), then
+// more elements a lane, then more waves: 16 elements a lane of x, dy, the weight, both sums and the next row are what leaves four waves
+// to a SIMD.  us forward / backward, taken and next best:
+//   262144 x 64 fp32           4 elements of 16 lanes 22 / 35       8 elements 28 / 39
+//   131072 x 128 bf16          8 elements of 16 lanes 14.5 / 22.6   2 elements of 64 lanes 34 / 35
+//   65536 x 256 bf16           16 elements of 16 lanes 12.6 / 24    4 elements of 64 lanes 20.7 / 26.5
+//   65536 x 256 fp32           4 elements of 64 lanes 22.4 / 35.9   16 elements of 16 lanes 21.7 / 35.7, but 1024 rows 3.0 / 6.3 against 2.5 / 5.4
+//   32768 x 512 bf16           8 elements of 64 lanes 15.7 / 24     16 elements 19 / 34
+//   16384 x 1024 bf16          one wave 13.6 / 23.4                 two waves 17 / 40
+//   16384 x 1100 bf16          two waves 24 forward, four 43 backward   four waves 32, two 49
+//   8192 x 4096 bf16           four waves 24 / 41                   eight waves 28 / 43
+//   4096 x 8192 bf16           eight waves 26 / 49                  sixteen waves 29 / 46
+//   2048 x 16384 bf16          sixteen waves 37 / 45                read again for each pass 82 / 129
+template <bool FORWARD, int SIZE, typename F>
 int with_shape(int64_t c, F&& f) {
     if (c <= 64) return f(Shape<16, 1, 4, 1>{});
-    if (c <= 128) return f(Shape<64, 1, 2, 1>{});
-    if (c <= 256) return f(Shape<64, 1, 4, 1>{});
+    if (c <= 128) return f(Shape<16, 1, 8, 1>{});
+    if (c <= 256) return f(std::conditional_t<SIZE == 2, Shape<16, 1, 8, 2>, Shape<64, 1, 4, 1>>{});
     if (c <= 512) return f(Shape<64, 1, 8, 1>{});
     if (c <= 1024) return f(Shape<64, 1, 8, 2>{});
     if (c <= 2048) return f(std::conditional_t<FORWARD, Shape<64, 2, 8, 2>, Shape<64, 4, 8, 1>>{});
@@ -421,9 +432,10 @@ int with_shape(int64_t c, F&& f) {
 // that the slices (8 bytes a column each) stay a small part of the rows' own traffic and do not wait for one another.  (us at 256 / 512 /
 // 768 / 1024 of them: 65536 x 256 fp32 53 / 36.5 / 35.5 / 35.5, 16384 x 1024 bf16 27 / 23 / 23.5 / 25.6, 16384 x 2048 bf16 72 / 44 / 40 / 39,
 // 8192 x 4096 bf16 51 / 43 / 42 / 46, 8192 x 8192 bf16 98 / 94 / 110 / 110, 4096 x 16384 fp32 164 / 181 / 192 / 207)
+template <int SIZE>
 int slices_of(int64_t n, int64_t c) {
     if (n < 1) return 1;
-    const int rows = c > LN_HELD ? 1 : with_shape<false>(c, [](auto s) { return decltype(s)::ROWS; });
+    const int rows = c > LN_HELD ? 1 : with_shape<false, SIZE>(c, [](auto s) { return decltype(s)::ROWS; });
     const int64_t groups = (n + rows - 1) / rows;
     const int64_t most = c <= 512 || (c > 1024 && c <= 2048) ? LN_SLICES : c > 2048 && c <= 4096 ? LN_SLICES * 3 / 4 : c <= 8192 ? LN_SLICES / 2 : LN_SLICES / 4;
     return (int)(groups < most ? groups : most);
@@ -438,7 +450,7 @@ int fwd(int64_t n, int c, const void* x, int64_t ldx, int w_f32, const void* w, 
                            (T*)y, ldy, stats);
         return launched("nerf_layer_norm_fwd");
     }
-    return with_shape<true>(c, [&](auto shape) {
+    return with_shape<true, sizeof(T)>(c, [&](auto shape) {
         using S = decltype(shape);
         const int64_t groups = (n + S::ROWS - 1) / S::ROWS;
         hipLaunchKernelGGL((k_ln_fwd_held<T, S>), dim3((unsigned)(groups < LN_GROUPS ? groups : LN_GROUPS)), dim3(S::THREADS), 0, stream, n, c, (const T*)x,
@@ -451,7 +463,7 @@ template <typename T>
 int bwd(int64_t n, int c, const void* x, int64_t ldx, const void* dy, int64_t lddy, int w_f32, const void* w, const float* stats, void* dx,
         int64_t lddx, void* dw, void* db, float* ws, hipStream_t stream) {
     const Param<T> wp{w, w_f32};
-    const int slices = slices_of(n, c);
+    const int slices = slices_of<sizeof(T)>(n, c);
     float* part = dw || db ? ws : nullptr;
     if (!dx && !part) return 0;
     int rc = 0;
@@ -469,7 +481,7 @@ int bwd(int64_t n, int c, const void* x, int64_t ldx, const void* dy, int64_t ld
             rc = launched("nerf_layer_norm_bwd (partial sums)");
         }
     } else {
-        rc = with_shape<false>(c, [&](auto shape) {
+        rc = with_shape<false, sizeof(T)>(c, [&](auto shape) {
             using S = decltype(shape);
             hipLaunchKernelGGL((k_ln_bwd_held<T, S>), dim3((unsigned)slices), dim3(S::THREADS), 0, stream, n, c, (const T*)x, ldx, (const T*)dy,
                                lddy, wp, stats, (T*)dx, lddx, part);
@@ -504,7 +516,7 @@ int nerf_layer_norm_fwd(int64_t n, int64_t c, int type, const void* x, int64_t l
 #undef GO
 }
 
-int64_t nerf_layer_norm_workspace_floats(int64_t n, int64_t c) { return c < 1 ? 0 : (int64_t)slices_of(n, c) * 2 * c; }
+int64_t nerf_layer_norm_workspace_floats(int64_t n, int64_t c) { return c < 1 ? 0 : (int64_t)std::max(slices_of<2>(n, c), slices_of<4>(n, c)) * 2 * c; }
 
 int nerf_layer_norm_bwd(int64_t n, int64_t c, int type, const void* x, int64_t ldx, const void* dy, int64_t lddy, int w_type,
                         const void* w, const float* stats, void* dx, int64_t lddx, void* dw, void* db, float* workspace, void* stream_) {

@@ -61,7 +61,7 @@ def _data(n, c, dtype, device, seed, offset=1.0, pad=0):
 
 SHAPES = [(1, 1), (3, 1), (2, 2), (1, 7), (5, 63), (7, 64), (4, 65), (65, 100), (33, 256), (1, 255), (300, 257), (9, 512), (2, 1000),
           (17, 1024), (5, 1025), (6, 1537), (3, 2048), (2, 2049), (4, 4096), (3, 5000), (2, 8192), (1, 8200), (2, 16384), (1, 20001),
-          (2, 33000), (1, 70001), (2000, 8), (5000, 3), (1031, 96), (700, 640)]
+          (2, 33000), (1, 70001), (2000, 8), (5000, 3), (1031, 96), (700, 640), (20011, 128), (17, 129), (9001, 200), (30000, 256)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
@@ -84,7 +84,7 @@ def test_forward_and_gradients(device, n, c, dtype):
             assert torch.equal(ops.layer_norm(xl, wl, bl), y)
 
 
-@pytest.mark.parametrize("n,c,pad", [(50, 257, 3), (33, 256, 64), (20, 1537, 63), (9, 4096, 8), (5, 8192, 1), (3, 20000, 5)])
+@pytest.mark.parametrize("n,c,pad", [(50, 257, 3), (33, 256, 64), (70, 127, 1), (300, 131, 2), (20, 1537, 63), (9, 4096, 8), (5, 8192, 1), (3, 20000, 5)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 def test_row_strides_and_missing_parameters(device, n, c, pad, dtype):
     """Rows that are a slice of a wider buffer (starting at any address), a transposed input, a broadcast gradient; weight or bias missing."""

@@ -11,6 +11,7 @@ import os
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import check, lib
 
@@ -967,6 +968,22 @@ def _launch(dev: torch.device, name: str, units: int, fn, *args) -> None:
         check(fn(*args, _stream()))
 
 
+# A call that no input wants a gradient of goes to the library without an autograd function (which costs several microseconds).  What
+# follows torch's operations from outside -- a trace (torch.jit.trace), forward-mode differentiation -- does not see such a launch: a
+# trace would keep the empty result alone, and a tangent would be dropped.  Such a call takes the autograd function: it is one
+# node of the trace, and a tangent is refused.
+def _followed() -> bool:
+    return torch._C._get_tracing_state() is not None or forward_ad._current_level >= 0
+
+
+class _Followed(torch.autograd.Function):
+    """fn(*tensors), a call that has no backward pass, for whoever follows it (see _followed)."""
+
+    @staticmethod
+    def forward(ctx, fn, *tensors):
+        return fn(*tensors)
+
+
 def _differentiable_once(backward):
     """torch.autograd.function.once_differentiable, paid for only where a graph of the backward pass is asked for."""
     guarded = torch.autograd.function.once_differentiable(backward)
@@ -1034,7 +1051,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     gradients are summed in a fixed order (bitwise reproducible)."""
     if not eps >= 0.0:
         raise ValueError(f"layer_norm: eps={eps}")
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+    if _followed() or torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                                   or (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _layer_norm_forward(x, weight, bias, float(eps), False)[0]
 
@@ -1052,7 +1070,7 @@ class Fp8Rows:
             raise ValueError(f"Fp8Rows: k={k}, codes {tuple(codes.shape)}, scales {tuple(scales.shape)}")
         if codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.uint8:
             raise TypeError(f"Fp8Rows: expected float8_e4m3fn codes and uint8 scales, got {codes.dtype} and {scales.dtype}")
-        rows = codes.shape[0]
+        rows = int(codes.shape[0])      # (a trace's sizes are tensors)
         want = (rows, int(lib.nerf_fp8_code_stride(k))), (rows, int(lib.nerf_fp8_scale_stride(k)))
         if (tuple(codes.shape), tuple(scales.shape)) != want:
             raise ValueError(f"Fp8Rows: for k={k} expected codes {want[0]} and scales {want[1]}, got {tuple(codes.shape)} and "
@@ -1093,6 +1111,11 @@ def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
     becomes NaN.  What comes out is not part of x's graph (linear_fp8 quantises inside and is)."""
     if x.dim() != 2:
         raise ValueError(f"quantize_fp8: expected a matrix, got shape {tuple(x.shape)}")
+    if _followed():
+        def both(x):
+            q = _quantize(x, True, False)[0]
+            return q.codes, q.scales
+        return Fp8Rows(*_Followed.apply(both, x.detach()), x.shape[1])
     return _quantize(x.detach(), True, False)[0]
 
 
@@ -1110,6 +1133,14 @@ def matmul_fp8(a: Fp8Rows, b: Fp8Rows, bias: Optional[torch.Tensor] = None, relu
     dev = a.codes.device
     if b.codes.device != dev:
         raise TypeError(f"matmul_fp8: operands on {dev} and {b.codes.device}")
+    if _followed():
+        return _Followed.apply(lambda ac, sa, bc, sb, bias: _matmul(Fp8Rows(ac, sa, a.k), Fp8Rows(bc, sb, b.k), bias, relu, out_dtype),
+                               a.codes, a.scales, b.codes, b.scales, bias)
+    return _matmul(a, b, bias, relu, out_dtype)
+
+
+def _matmul(a: Fp8Rows, b: Fp8Rows, bias, relu: bool, out_dtype: torch.dtype) -> torch.Tensor:
+    dev = a.codes.device
     c = torch.empty((a.rows, b.rows), dtype=out_dtype, device=dev)
     bias = _vector(bias, b.rows, c, "bias")
     kind = ELEM_TYPES[out_dtype]
@@ -1192,12 +1223,15 @@ def linear_fp8(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = None, rel
             raise ValueError(f"linear_fp8: x {tuple(x.shape)} against a weight with k={weight.k}")
         if weight.codes.device != x.device:
             raise TypeError(f"linear_fp8: x on {x.device}, the weight on {weight.codes.device}")
+        if _followed():
+            return _Followed.apply(lambda x, codes, scales, b: _linear_fp8_forward(x, Fp8Rows(codes, scales, weight.k), b, bool(relu), False, False)[0],
+                                   x, weight.codes, weight.scales, bias)
         return _linear_fp8_forward(x, weight, bias, bool(relu), False, False)[0]
     _elem(x, "x")
     if weight.dim() != 2 or x.dim() < 1 or weight.shape[1] != x.shape[-1]:
         raise ValueError(f"linear_fp8: x {tuple(x.shape)} against weight {tuple(weight.shape)}")
     if weight.device != x.device or weight.dtype not in (x.dtype, torch.float32):
         raise TypeError(f"linear_fp8: expected a weight in {x.dtype} or fp32 on {x.device}, got {weight.dtype} on {weight.device}")
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+    if _followed() or torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return _LinearFp8.apply(x, weight, bias, bool(relu))
     return _linear_fp8_forward(x, weight, bias, bool(relu), False, False)[0]

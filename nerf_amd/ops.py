@@ -985,11 +985,16 @@ class _Followed(torch.autograd.Function):
 
 
 def _differentiable_once(backward):
-    """torch.autograd.function.once_differentiable, paid for only where a graph of the backward pass is asked for."""
-    guarded = torch.autograd.function.once_differentiable(backward)
-
+    """A backward pass that cannot be differentiated: where a graph of it is asked for, differentiating its results raises.
+    (torch.autograd.function.once_differentiable lets a result through as a constant where the incoming gradient needs none, so that the
+    second derivative in the saved inputs would be dropped without a word.)"""
     def run(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        raises = torch._C._functions.DelayedError(b"this operator is differentiable once: its gradients have no derivative", len(out))
+        return raises(*(t if t is None else t.detach().requires_grad_(True) for t in out))
     return run
 
 

@@ -1,5 +1,5 @@
-"""The layer operators where something follows torch's operations from outside: traces and forward-mode derivatives.  Here with the
-launch left out (what is recorded does not depend on it); on the GPU the traced calls are run on other inputs."""
+"""The layer operators where something follows torch's operations from outside: traces, forward-mode and second derivatives.  Here with
+the launch left out (what is recorded does not depend on it); on the GPU the traced calls are run on other inputs."""
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -45,6 +45,20 @@ def test_a_tangent_is_not_dropped(launches, i):
             f(forward_ad.make_dual(x, torch.ones_like(x)))
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward mode AD"):
             f(forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_a_second_derivative_is_refused(launches, i):
+    _, f = _calls()[i]
+    x = torch.randn(3, 8, requires_grad=True)
+    dy = torch.randn_like(f(x)).requires_grad_(True)
+    for incoming in (dy, dy.detach()):           # (the first gradient depends on x either way)
+        (dx,) = torch.autograd.grad(f(x), x, incoming, create_graph=True)
+        assert dx.shape == x.shape
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            (f(x).sum() + (dx ** 2).sum()).backward()
+    (dx,) = torch.autograd.grad(f(x), x, dy)
+    assert not dx.requires_grad
 
 
 @pytest.mark.gpu

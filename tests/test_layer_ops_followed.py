@@ -61,6 +61,15 @@ def test_a_second_derivative_is_refused(launches, i):
     assert not dx.requires_grad
 
 
+def test_a_graph_of_torch_operations_is_refused(monkeypatch):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from nerf_amd import ops
+    monkeypatch.setattr(ops, "_elem", lambda t, what: ops.ELEM_TYPES[t.dtype])
+    for _, f in _calls():
+        with pytest.raises(RuntimeError, match="cannot be recorded"):
+            make_fx(f)(torch.randn(3, 8))
+
+
 @pytest.mark.gpu
 def test_traced_calls_on_other_inputs(device):
     """With weights of either kind, and every step of a product in 8 bits: the trace computes what the call does."""

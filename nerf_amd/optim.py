@@ -374,7 +374,7 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         states = list(self.state.values())
         known = len(states) == len(self._seen) and all(map(operator.is_, states, self._seen))
-        work = []
+        work, written = [], []
         for group in self.param_groups:      # (everything is checked before anything is launched)
             self._check_hyper(group["lr"], group["betas"], group["eps"], group["weight_decay"])
             grads = list(map(_grad, group["params"]))
@@ -387,7 +387,9 @@ class AdamW(torch.optim.Optimizer):
                     if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != launch.device:
                         raise TypeError(f"AdamW: a device learning rate must be one fp32 value on {launch.device}, got {lr.dtype} on {lr.device}")
             work += [(group, launch, launch.take(grads)) for launch in plan.launches]
+            written += plan.pointed
         self._seen = list(self.state.values())
+        torch.autograd.graph.increment_version(written)      # (a graph that saved a parameter refuses its backward pass from here on)
         for group, launch, (addresses, _) in work:
             self._launch(group, launch, addresses)
         return loss

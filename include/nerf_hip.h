@@ -410,9 +410,10 @@ int nerf_layer_norm_bwd(int64_t n, int64_t c, int type, const void* x, int64_t l
  *   columns of the (masked) x; it takes a workspace of nerf_fp8_quantize_workspace_floats(rows, cols) floats.  (mask without col_sum
  *   is allowed; rows and columns behind the last are not read.)
  * nerf_fp8_matmul: c [m, n] of `type`, row stride ldc, = act(a [m, k] b [n, k]^T + bias [n]); bias (of bias_type: `type` or
- *   NERF_F32) may be NULL; relu != 0 applies max(., 0) (a NaN stays).  Sums in fp32: for an fp32 c by the bf16 matrix instruction
- *   on decoded values (products exact), for a 16-bit c by the scaled fp8 instruction, which cuts the products of eight consecutive
- *   k to multiples of 2^-13 of the largest one's power of two (typically 1.5e-5 of the result).
+ *   NERF_F32) may be NULL; relu != 0 applies max(., 0) (a NaN stays).  Sums in fp32 by the bf16 matrix instruction on decoded values: products
+ *   are exact for values of magnitude from 2^-126 to below 2^128 (smaller ones may count as 0, larger ones as infinite; a scale byte of 255 makes its
+ *   block NaN).  For a bf16 c of more than a few rows by the scaled 8-bit instruction, which cuts the products of eight consecutive k to
+ *   multiples of 2^-13 of the largest one's power of two: 1.5e-5 to 7.5e-5 of the result (rms), at most 7 * 2^-13 of sum |a b|.
  *   workspace: nerf_fp8_matmul_workspace_floats(m, n, k, type) floats (0: may be NULL). */
 int64_t nerf_fp8_code_stride(int64_t k);
 int64_t nerf_fp8_scale_stride(int64_t k);

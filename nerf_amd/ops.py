@@ -1129,7 +1129,9 @@ def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
 
 def matmul_fp8(a: Fp8Rows, b: Fp8Rows, bias: Optional[torch.Tensor] = None, relu: bool = False,
                out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """a [m, k] b [n, k]^T + bias [n] (+ ReLU) in out_dtype (fp32, bf16 or fp16); sums in fp32.  No backward pass."""
+    """a [m, k] b [n, k]^T + bias [n] (+ ReLU) in out_dtype (fp32, bf16 or fp16).  Sums in fp32 of exact products; for bf16 and more than a
+    few rows by the 8-bit matrix instruction, which is twice as fast and keeps 13 bits below the largest of every eight products (a
+    result that cancels almost wholly loses by that: take fp32 there).  No backward pass."""
     if bias is not None and bias.requires_grad and torch.is_grad_enabled():
         raise ValueError("matmul_fp8: no backward pass for the bias; call it under torch.no_grad()")
     if not (isinstance(a, Fp8Rows) and isinstance(b, Fp8Rows)):
@@ -1223,7 +1225,7 @@ def linear_fp8(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = None, rel
     """ops.linear with both operands of every product held in 8 bits, one power-of-two scale per row and 128 values of k.
     x [..., k]: fp32, bf16 or fp16, and the result's type.  weight: a tensor [n, k] of x's type or fp32 -- quantised in the call,
     differentiable once in x, weight and bias (each product of the backward pass in 8 bits as well) -- or an Fp8Rows (kept by a
-    program that only evaluates; no gradients).  Sums are fp32."""
+    program that only evaluates; no gradients).  Each product's sums are matmul_fp8's for its result's type."""
     if isinstance(weight, Fp8Rows):
         if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
             raise ValueError("linear_fp8: a weight held in 8 bits has no backward pass; call it under torch.no_grad()")

@@ -414,7 +414,8 @@ int nerf_layer_norm_bwd(int64_t n, int64_t c, int type, const void* x, int64_t l
  *   are exact for values of magnitude from 2^-126 to below 2^128 (smaller ones may count as 0, larger ones as infinite; a scale byte of 255 makes its
  *   block NaN).  For a bf16 c of more than a few rows by the scaled 8-bit instruction, which cuts the products of eight consecutive k to
  *   multiples of 2^-13 of the largest one's power of two: 1.5e-5 to 7.5e-5 of the result (rms), at most 7 * 2^-13 of sum |a b|.
- *   workspace: nerf_fp8_matmul_workspace_floats(m, n, k, type) floats (0: may be NULL). */
+ *   workspace: nerf_fp8_matmul_workspace_floats(m, n, k, type) floats (0: may be NULL).  nerf_fp8_matmul_tile tells which kernel takes
+ *   the product: 0 the one for few rows, otherwise the edge of its tiles. */
 int64_t nerf_fp8_code_stride(int64_t k);
 int64_t nerf_fp8_scale_stride(int64_t k);
 int64_t nerf_fp8_quantize_workspace_floats(int64_t rows, int64_t cols);
@@ -422,6 +423,7 @@ int nerf_fp8_quantize(int64_t rows, int64_t cols, int type, const void* x, int64
                       uint8_t* codes, uint8_t* scales, uint8_t* codes_t, uint8_t* scales_t, int sum_type, void* col_sum,
                       float* workspace, void* stream);
 int64_t nerf_fp8_matmul_workspace_floats(int64_t m, int64_t n, int64_t k, int type);
+int nerf_fp8_matmul_tile(int64_t m, int64_t n, int64_t k, int type);
 int nerf_fp8_matmul(int64_t m, int64_t n, int64_t k, const uint8_t* a, const uint8_t* a_scales, const uint8_t* b,
                     const uint8_t* b_scales, int bias_type, const void* bias, int relu, int type, void* c, int64_t ldc,
                     float* workspace, void* stream);

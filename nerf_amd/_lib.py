@@ -100,6 +100,7 @@ SIGNATURES = {
     "nerf_fp8_quantize_workspace_floats": (_l, [_l, _l]),
     "nerf_fp8_quantize": (_i, [_l, _l, _i, _p, _l, _p, _l, _p, _p, _p, _p, _i, _p, _p, _p]),
     "nerf_fp8_matmul_workspace_floats": (_l, [_l, _l, _l, _i]),
+    "nerf_fp8_matmul_tile": (_i, [_l, _l, _l, _i]),
     "nerf_fp8_matmul": (_i, [_l, _l, _l, _p, _p, _p, _p, _i, _p, _i, _i, _p, _l, _p, _p]),
     "nerf_linear_fp8_kept_bytes": (_l, [_l, _l, _l, _i, _i]),
     "nerf_linear_fp8_workspace_bytes": (_l, [_l, _l, _l, _i, _i, _i]),

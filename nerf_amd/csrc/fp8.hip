@@ -961,6 +961,8 @@ int nerf_fp8_matmul(int64_t m, int64_t n, int64_t k, const uint8_t* a, const uin
     return product<f16_t>(p, k, type, workspace, stream);
 }
 
+int nerf_fp8_matmul_tile(int64_t m, int64_t n, int64_t k, int type) { return m < 1 || n < 1 || k < 1 ? 0 : plan_of(m, n, k, type).tile; }
+
 int64_t nerf_fp8_matmul_workspace_floats(int64_t m, int64_t n, int64_t k, int type) {
     if (m < 1 || n < 1 || k < 1) return 0;
     const Plan plan = plan_of(m, n, k, type);

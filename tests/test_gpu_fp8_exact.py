@@ -8,7 +8,6 @@ import torch
 
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 IDS = ["f32", "bf16", "f16"]
-CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 def _whole(rows, k, top, device, seed):
@@ -28,6 +27,39 @@ def _would_show(a, b, want, out):
     for kb in {0, blocks // 2, blocks - 1}:
         part = slice(128 * kb, 128 * (kb + 1))
         assert not torch.equal((want - _product(a[:, part], b[:, part])).to(out), want.to(out)), kb
+
+
+# (m, n, k) -> blocks of k 7, 9, 10, 11, 12, 13 (the image a tile starts in goes by the count's parity, its words of scales by the
+# count / 4 rounded up); two and three tiles a workgroup, the last round full and not; fewer tiles than workgroups
+LARGE = [(4096, 8192, 896), (4096, 8192, 1100), (4090, 8187, 1280), (6100, 8190, 1400), (5120, 8192, 1536), (4096, 8100, 1601), (4608, 8192, 2100),
+         (2560, 3584, 4096), (2500, 3500, 2200), (3840, 4000, 1900)]
+
+
+def test_the_large_cases_take_large_tiles():
+    from nerf_amd._lib import lib
+    for m, n, k in LARGE:
+        assert lib.nerf_fp8_matmul_tile(m, n, k, 1) == 256, (m, n, k)
+        assert lib.nerf_fp8_matmul_tile(m, n, k, 0) == lib.nerf_fp8_matmul_tile(m, n, k, 2) == 128
+    tiles = [(-(-m // 256)) * (-(-n // 256)) for m, n, _ in LARGE]
+    assert min(tiles) < 256 and max(tiles) > 512 and any(t % 256 for t in tiles if t > 256)
+    assert {-(-k // 128) % 4 for _, _, k in LARGE} == {0, 1, 2, 3}
+    assert lib.nerf_fp8_matmul_tile(4, 8192, 8192, 1) == 0 and lib.nerf_fp8_matmul_tile(0, 1, 1, 1) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", LARGE)
+def test_large_tiles(device, m, n, k):
+    """bf16, with a bias and without, and the call's repetition."""
+    from nerf_amd import ops
+    a, b = _whole(m, k, 4, device, m), _whole(n, k, 4, device, n + 1)
+    assert 16 * k < 2 ** 24
+    want = _product(a, b)
+    _would_show(a, b, want, torch.bfloat16)
+    qa, qb = ops.quantize_fp8(a), ops.quantize_fp8(b)
+    bias = _whole(1, n, 4, device, 5)[0]
+    for _ in range(2):
+        assert torch.equal(ops.matmul_fp8(qa, qb, out_dtype=torch.bfloat16), want.bfloat16())
+        assert torch.equal(ops.matmul_fp8(qa, qb, bias, True, torch.bfloat16), (want + bias.double()).clamp_min(0).bfloat16())
 
 
 @pytest.mark.gpu

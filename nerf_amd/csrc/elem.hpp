@@ -11,12 +11,6 @@ namespace nerfhip {
 typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 
-template <typename T> struct ElemTraits;
-template <> struct ElemTraits<float> { static constexpr int code = 0; };
-template <> struct ElemTraits<bf16_t> { static constexpr int code = 1; };
-template <> struct ElemTraits<f16_t> { static constexpr int code = 2; };
-
-inline int elem_size(int type) { return type == 0 ? 4 : 2; }
 inline bool elem_type_ok(int type) { return type >= 0 && type <= 2; }
 
 // N consecutive elements from any element's address: the memory system takes vector accesses at any alignment, so that odd strides and

@@ -822,34 +822,36 @@ struct Plan {
     int tile;           // 0: few rows; else the tile's edge
     int slices;         // of k
     int blocks_per_slice;
-    int units;          // compute units: workgroups that stay for several large tiles
 };
+// The machine's compute units, which cut a product and are the most workgroups that stay for several large tiles.  A constant and not the
+// current device's count: workspaces are sized without a device, and the same product gives the same bits on every one (on a
+// partition of the machine with fewer of them the workgroups take turns).
+constexpr int UNITS = 256;
 Plan plan_of(int64_t m, int64_t n, int64_t k, int type) {
     const int64_t blocks = blocks_of(k);
     // Few rows or tiles: what either takes in us, fitted to both at 4 to 64 rows and n x k from 256 x 256 to 8192 x 8192 and 1024 x 65536.
     // (8192 x 8192: 4 rows 13.9 / 17.4, 16 rows 18.6 / 18.1, 64 rows 42.8 / 20.9; 1024 x 1024, 64 rows: 5.5 / 8.9;
     // 1024 x 65536, 4 rows: 47 / 18, few workgroups with a long way each)
     const double few = 2.4 + (double)k * (n > 4096 ? n : 4096) * (17 + m) / 1.34e8, many = 7.5 + (double)n * k / 6.4e6;
-    if ((m <= 64 && few <= many) || k > (1 << 22)) return {0, 1, (int)blocks, 0};
+    if ((m <= 64 && few <= many) || k > (1 << 22)) return {0, 1, (int)blocks};
     auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
-    const int cus = 256;
     const int64_t small = tiles(128);
     // Large tiles or small: large ones use the matrix instruction better, and a tile costs them more.  What either takes in us, fitted to
     // 2048 x 2048 to 5632 x 5632 at k = 4096 and 512 and to 65536 x 256 x 256; a round that is not full takes less than a full one.  (16 bits,
     // large / small: 4096 x 4096 x 4096 62 / 74, 2560 x 3584 x 4096 45 / 55, 5632 x 5632 x 4096 105 / 135, 2048 x 2048 x 4096 61 / 26,
     // 4096 x 4096 x 512 19.5 / 17.2.)  Large tiles ask for blocks two ahead, so that they need two.
-    const double r = (double)tiles(256) / cus, q = (double)small / (2 * cus);
+    const double r = (double)tiles(256) / UNITS, q = (double)small / (2 * UNITS);
     const double large_us = (r + 2 * std::ceil(r)) / 3 * (13.4 + 1.3 * blocks), small_us = (q + std::ceil(q)) / 2 * (4.5 + 1.02 * blocks);
-    if (type == NERF_BF16 && blocks > 1 && large_us < small_us) return {256, 1, (int)blocks, cus};
+    if (type == NERF_BF16 && blocks > 1 && large_us < small_us) return {256, 1, (int)blocks};
     // Few small tiles leave compute units idle: k is cut in slices, whose sums a second launch joins.  A block takes 0.76 us, the join
     // 5 us and what the partial sums cost to write and to read.  (256 x 256 x 65536 fp32: 1 slice 390, 16 slices 34.5, 64 slices 21.0;
     // 1024 x 1024 x 1024: 1 slice 7.3, 2 slices 12.6.)
-    const int64_t most = small < cus ? std::min(cus / small, blocks) : 1;
+    const int64_t most = small < UNITS ? std::min(UNITS / small, blocks) : 1;
     const double block_us = 0.76, sum_us = 2e-6 * (double)m * n;
     int64_t slices = std::min(std::max((int64_t)(std::sqrt(blocks * block_us / sum_us) + 0.5), (int64_t)1), most);
     if (blocks * block_us / slices + 5 + slices * sum_us >= blocks * block_us) slices = 1;
     const int64_t per = (blocks + slices - 1) / slices;
-    return {128, (int)((blocks + per - 1) / per), (int)per, cus};
+    return {128, (int)((blocks + per - 1) / per), (int)per};
 }
 
 template <typename T>
@@ -866,7 +868,7 @@ int product(const Product& p, int64_t k, int type, float* ws, hipStream_t stream
     }
     const int64_t tm = (p.m + plan.tile - 1) / plan.tile, tn = (p.n + plan.tile - 1) / plan.tile;
     if (tm * tn > 0xffffff) return fail(NERF_E_ARG, "nerf_fp8_matmul: %lld x %lld is more than one launch covers", (long long)p.m, (long long)p.n);
-    const int64_t wgs = plan.tile == 256 && tm * tn > plan.units ? plan.units : tm * tn;
+    const int64_t wgs = plan.tile == 256 && tm * tn > UNITS ? UNITS : tm * tn;
     const dim3 grid((unsigned)wgs, 1, (unsigned)plan.slices);
     float* part = plan.slices > 1 ? ws : nullptr;
     if (plan.slices > 1 && !ws) return fail(NERF_E_ARG, "nerf_fp8_matmul: null workspace");

@@ -912,7 +912,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], 
 # layers of wide networks: layer norm, products in 8 bits
 # ------------------------------------------------------------------------------------------------
 _empty_like, _CONTIGUOUS = torch.empty_like, torch.contiguous_format
-_dispatch_mode, _PROXY = torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY
+_tracing_state, _dispatch_modes = torch._C._get_tracing_state, torch._C._len_torch_dispatch_stack
 # (the library's size queries depend on their arguments alone; a call through ctypes costs more than looking its answer up)
 _layer_norm_workspace, _matmul_workspace, _linear_kept, _linear_workspace = (
     functools.lru_cache(maxsize=1024)(f) for f in (lib.nerf_layer_norm_workspace_floats, lib.nerf_fp8_matmul_workspace_floats,
@@ -956,8 +956,6 @@ def _vector(t: Optional[torch.Tensor], size: int, like: torch.Tensor, what: str)
 # A launch on the tensors' device and its current stream, bracketed with events when PROFILE is a list.  (Torch's device context and
 # stream objects cost several microseconds each, which a call of a few microseconds would spend twice over.)
 def _launch(dev: torch.device, name: str, units: int, fn, *args) -> None:
-    if _dispatch_mode(_PROXY) is not None:      # (make_fx: its graph would hold the empty result alone)
-        raise RuntimeError(f"{name}: a launch cannot be recorded as a graph of torch operations")
     if dev.index == torch.cuda.current_device():
         if PROFILE is None:
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
@@ -974,9 +972,11 @@ def _launch(dev: torch.device, name: str, units: int, fn, *args) -> None:
 # A call that no input wants a gradient of goes to the library without an autograd function (which costs several microseconds).  What
 # follows torch's operations from outside -- a trace (torch.jit.trace), forward-mode differentiation -- does not see such a launch: a
 # trace would keep the empty result alone, and a tangent would be dropped.  Such a call takes the autograd function: it is one
-# node of the trace, and a tangent is refused.
+# node of the trace, and a tangent is refused.  A graph of torch operations (make_fx) has no place for it, with or without the function.
 def _followed() -> bool:
-    return torch._C._get_tracing_state() is not None or forward_ad._current_level >= 0
+    if _dispatch_modes() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError("a layer operator cannot be recorded as a graph of torch operations")
+    return forward_ad._current_level >= 0 or _tracing_state() is not None
 
 
 class _Followed(torch.autograd.Function):

@@ -387,7 +387,7 @@ class AdamW(torch.optim.Optimizer):
                     if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != launch.device:
                         raise TypeError(f"AdamW: a device learning rate must be one fp32 value on {launch.device}, got {lr.dtype} on {lr.device}")
             work += [(group, launch, launch.take(grads)) for launch in plan.launches]
-            written += plan.pointed
+            written += plan.live
         self._seen = list(self.state.values())
         torch.autograd.graph.increment_version(written)      # (a graph that saved a parameter refuses its backward pass from here on)
         for group, launch, (addresses, _) in work:

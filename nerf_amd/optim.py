@@ -64,6 +64,8 @@ class FlatAdam(torch.optim.Adam):
         """What does not change from step to step: the update rule and the parameters' type and placement."""
         if group.get("amsgrad") or group.get("maximize") or group.get("differentiable") or not group["params"]:
             return False
+        if group.get("decoupled_weight_decay") and group["weight_decay"]:      # (from a checkpoint of AdamW; the kernel's decay is Adam's)
+            return False
         return all(p.is_cuda and p.dtype == torch.float32 and p.is_contiguous() for p in group["params"])
 
     def _find_runs(self):
@@ -197,7 +199,8 @@ class FlatAdam(torch.optim.Adam):
 
     def load_state_dict(self, state_dict):
         """As torch.optim.Adam, for checkpoints of either optimiser (and of upstream's); the groups keep this class's
-        fused / capturable settings whatever the checkpoint's were, so that the stock step stays usable on the state."""
+        fused / capturable settings whatever the checkpoint's were, so that the stock step stays usable on the state.  A checkpoint of
+        AdamW goes on with its decoupled weight decay (the stock step has it)."""
         super().load_state_dict(state_dict)
         for group in self.param_groups:
             group["fused"], group["capturable"], group["foreach"] = True, True, None
@@ -312,7 +315,8 @@ class AdamW(torch.optim.Optimizer):
         self._check_hyper(lr, betas, eps, weight_decay)
         self.state_bits = state_bits
         self._plans, self._seen = {}, []      # what the last step looked up: see _Plan
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, capturable=True))
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, capturable=True,
+                                      decoupled_weight_decay=True))      # (for Adam's classes, should they load a checkpoint of this one)
 
     @staticmethod
     def _check_hyper(lr, betas, eps, weight_decay):
@@ -437,7 +441,7 @@ class AdamW(torch.optim.Optimizer):
             fresh[p] = new
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         for group in self.param_groups:
-            group["capturable"] = True
+            group["capturable"] = group["decoupled_weight_decay"] = True
         self._plans, self._seen = {}, []
         for p, new in fresh.items():
             self.state[p] = new

@@ -200,7 +200,9 @@ class FlatAdam(torch.optim.Adam):
     def load_state_dict(self, state_dict):
         """As torch.optim.Adam, for checkpoints of either optimiser (and of upstream's); the groups keep this class's
         fused / capturable settings whatever the checkpoint's were, so that the stock step stays usable on the state.  A checkpoint of
-        AdamW goes on with its decoupled weight decay (the stock step has it)."""
+        AdamW goes on with its decoupled weight decay (the stock step has it); one with states in 8 bits is refused."""
+        if any("scale" in st for st in state_dict["state"].values()):
+            raise ValueError("FlatAdam: a checkpoint of AdamW with states in 8 bits (state_bits = 8)")
         super().load_state_dict(state_dict)
         for group in self.param_groups:
             group["fused"], group["capturable"], group["foreach"] = True, True, None

@@ -12,6 +12,18 @@ def _flat(params, **kw):
     return FlatAdam(params, lr=1.0, **kw)
 
 
+def test_eight_bit_states_are_not_taken_for_plain_ones():
+    """Their codes without their scales would be moments of another size."""
+    p = torch.nn.Parameter(torch.zeros(200))
+    ckpt = {"state": {0: {"step": torch.tensor(3.0), "exp_avg": torch.zeros(200, dtype=torch.uint8).view(torch.float8_e4m3fn),
+                          "exp_avg_sq": torch.zeros(200, dtype=torch.uint8).view(torch.float8_e5m2), "scale": torch.ones(2, 2)}},
+            "param_groups": [dict(lr=LR, betas=BETAS, eps=EPS, weight_decay=WD, capturable=True, params=[0])]}
+    opt = _flat([p])
+    with pytest.raises(ValueError, match="8 bits"):
+        opt.load_state_dict(ckpt)
+    assert not opt.state and opt.param_groups[0]["lr"] == 1.0
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("decay", [0.0, WD])
 @pytest.mark.parametrize("to", ["FlatAdam", "torch.Adam", "torch.AdamW", "AdamW"])

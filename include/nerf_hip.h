@@ -451,7 +451,7 @@ int nerf_linear_fp8_bwd(int64_t n, int64_t n_in, int64_t n_out, int type, const 
  * at params[i], gradients at grads[i], *steps[i] (a float) the number of updates taken so far, incremented by the call:
  *   m += (1 - beta1)(g - m), v += (1 - beta2)(g g - v), p -= lr wd p + lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps).
  * state_bits 32: exp_avg[i], exp_avg_sq[i] are fp32.  state_bits 8: exp_avg[i] e4m3 and exp_avg_sq[i] e5m2 bytes, scales[i] two
- * floats (max |m| / 448, max v / 57344) per block of 128 consecutive elements; the states are rounded stochastically, from a hash
+ * floats (max |m| / 448, max v / 57344, at least 1e-38 unless all are 0) per block of 128 consecutive elements; the states are rounded stochastically, from a hash
  * of (element, step).  type 16-bit: masters[i] are fp32 copies the parameters are rounded from (an element of params that no
  * longer equals its rounded master is taken as it is).  Tensors must not overlap.  lr_dev: the learning rate as a DEVICE float, or NULL and `lr` is used.
  * workspace: nerf_adamw_workspace_floats(n_tensors) floats, 16-byte aligned.  One launch per NERF_ADAMW_BATCH tensors and

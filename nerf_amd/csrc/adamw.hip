@@ -5,8 +5,8 @@
 // in fp32 (the moments as increments, so that their fixed point does not depend on how beta rounds); 16-bit parameters are
 // rounded from an fp32 master copy.
 //
-// States in 8 bits: per block of 128 consecutive elements of a tensor the scales sm = max |m| / 448 and sv = max v / 57344 (fp32),
-// m / sm held in e4m3 and v / sv in e5m2.  Both are rounded stochastically: with beta2 = 0.999 a step moves v by at most a
+// States in 8 bits: per block of 128 consecutive elements of a tensor the scales sm = max |m| / 448 and sv = max v / 57344 (fp32, at
+// least 1e-38 unless the block is 0), m / sm held in e4m3 and v / sv in e5m2.  Both are rounded stochastically: with beta2 = 0.999 a step moves v by at most a
 // thousandth of what it lacks, far below half a step of any 8-bit format, so that rounded to nearest it would stand still; rounded up with
 // the probability of the remainder its mean is kept.  The random bits are a hash of (element, step): the same run gives the
 // same bits.  A positive v never becomes 0, because it divides.
@@ -202,8 +202,14 @@ __global__ void __launch_bounds__(THREADS) k_adamw(Tensors ts, const Coef* __res
             am = mb > am ? mb : am;
             av = vb > av ? vb : av;
         }
-        const float sm = __uint_as_float(row_max(am)) * (1.0f / 448.0f), sv = __uint_as_float(row_max(av)) * (1.0f / 57344.0f);
-        const float dm = fmaxf(sm, 1e-38f), dv = fmaxf(sv, 1e-38f);
+        // (a scale is what the codes are divided by here and multiplied by in the next step: at least LEAST, unless all is 0)
+        constexpr float LEAST = 1e-38f;
+        am = row_max(am);
+        av = row_max(av);
+        float sm = __uint_as_float(am) * (1.0f / 448.0f), sv = __uint_as_float(av) * (1.0f / 57344.0f);
+        if (am && sm < LEAST) sm = LEAST;      // (a NaN stays)
+        if (av && sv < LEAST) sv = LEAST;
+        const float dm = fmaxf(sm, LEAST), dv = fmaxf(sv, LEAST);
         unsigned a[2] = {0, 0}, b[2] = {0, 0};
 #pragma unroll
         for (int e = 0; e < PER; ++e) {

@@ -302,7 +302,8 @@ class AdamW(torch.optim.Optimizer):
       step         fp32 scalar on the device
       exp_avg, exp_avg_sq   state_bits = 32: fp32, as torch.optim.AdamW's (whose checkpoints of fp32 parameters load, and the reverse);
                    state_bits = 8: float8_e4m3fn and float8_e5m2, relative to `scale`
-      scale        state_bits = 8: fp32 [blocks of 128 consecutive elements, 2]: the largest |exp_avg| / 448 and exp_avg_sq / 57344
+      scale        state_bits = 8: fp32 [blocks of 128 consecutive elements, 2]: the largest |exp_avg| / 448 and exp_avg_sq / 57344, at
+                   least 1e-38 unless all are 0
       master       16-bit parameters: the fp32 values they are rounded from (an element of the parameter that was written from
                    outside, and so is no longer its master's rounding, is taken as it is)
     8-bit states are rounded stochastically from a hash of (element, step), so a run repeats bit for bit; a gradient that is not

@@ -185,6 +185,13 @@ class NeRF(nn.Module):
         # to each weight matrix's largest gradient; the second also relative to every single entry
         self.dw_dtype = 'f16x2'
 
+    def __setstate__(self, state):
+        """Modules pickled whole before the options of wide networks existed come back without them."""
+        super().__setstate__(state)
+        self.__dict__.setdefault('layer_dtype', 'f32')
+        if 'pts_norms' not in self._modules:
+            self.__dict__.setdefault('pts_norms', None)
+
     # -- kernel plumbing ---------------------------------------------------------------------------
     def fused_arch(self) -> bool:
         """Whether the hand-written kernels cover this module's shape."""

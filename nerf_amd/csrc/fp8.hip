@@ -348,7 +348,7 @@ __device__ __forceinline__ f32x4 mul_decoded(i32x8 a, int sa, i32x8 b, int sb, f
 
 // Few rows: a workgroup owns 16 columns of C and up to 16 MT rows; each of its waves takes an eighth of the blocks of k, straight from
 // memory into the instruction's registers, four blocks requested at a time, and the waves add up through LDS.  The weight's codes
-// are read once: that is what bounds it (4 x 8192 x 8192 in 13.9 us, 4.9 TB/s).
+// are read once: that is what bounds it (4 x 8192 x 8192 in 13.9-14.3 us, 4.7-4.9 TB/s).
 constexpr int FEW_WAVES = 8, FEW_U = 4;
 template <typename T, int MT>
 __global__ void __launch_bounds__(64 * FEW_WAVES) k_product_few(Product p) {
@@ -538,9 +538,9 @@ struct TileLds {      // two images, two sets of scale words, a band of eight ro
 // one before it is still multiplied and written.  (A workgroup for each tile spent 11.5 us of 103 on the way out and in; bf16 of
 // 8192^3: 413 -> 390 us.)  Scales come once in four blocks: a word of a row costs the cache a lookup like a whole line, and with every
 // block they were half of them (8192 x 8192 x 16384: 848 -> 746 us).
-// 256 x 256, bf16 of random codes: 8192^3 in 385 us (2.86 PFLOP/s), 16384 x 8192 x 4096 in 418 us (2.63); of zeros 277 us -- the board's power
-// limit takes the rest, the matrix pipe is busy 81 % of the cycles, 15 % are waits at the two barriers of a block.  128 x 128, fp32: 8192^3
-// in 845 us (1.30 PFLOP/s, of the bf16 instruction), 65536 x 256 x 256 in 18-20 us (4.2-4.7 TB/s).
+// 256 x 256, bf16 of random codes: 8192^3 in 385-418 us over the boards (2.6-2.9 PFLOP/s), 16384 x 8192 x 4096 in 409-441 us; of zeros 277 us -- the board's power
+// limit takes the rest, the matrix pipe is busy 81 % of the cycles, 15 % are waits at the two barriers of a block.  128 x 128, fp32 and fp16:
+// 8192^3 in 845 us (1.30 PFLOP/s, of the bf16 instruction), 16384 x 8192 x 4096 in 917-934 us, 65536 x 256 x 256 in 18-20 us (4.2-4.7 TB/s).
 template <typename T, int BM, int BN>
 __global__ void __launch_bounds__(256) k_product_tile(Product p, int tiles_m, int tiles_n, int blocks_per_slice, float* __restrict__ partial) {
     constexpr bool DECODED = !std::is_same_v<T, bf16_t>;      // which instruction: see the top of this file
@@ -833,11 +833,13 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, int type) {
     // (8192 x 8192: 4 rows 13.9 / 17.4, 16 rows 18.6 / 18.1, 64 rows 42.8 / 20.9; 1024 x 1024, 64 rows: 5.5 / 8.9;
     // 1024 x 65536, 4 rows: 47 / 18, few workgroups with a long way each)
     const double few = 2.4 + (double)k * (n > 4096 ? n : 4096) * (17 + m) / 1.34e8, many = 7.5 + (double)n * k / 6.4e6;
+    // And a k above 2^22 whatever m and n, with 64-bit offsets throughout, where a tile's rows are 32 bits apart (they would reach to 2^24;
+    // 256 x 256 over 2^22 values of k by tiles 1.1 ms, over 2^22 + 300 by few rows 10.7 ms).
     if ((m <= 64 && few <= many) || k > (1 << 22)) return {0, 1, (int)blocks};
     auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
     const int64_t small = tiles(128);
     // Large tiles or small: large ones use the matrix instruction better, and a tile costs them more.  What either takes in us, fitted to
-    // 2048 x 2048 to 5632 x 5632 at k = 4096 and 512 and to 65536 x 256 x 256; a round that is not full takes less than a full one.  (16 bits,
+    // 2048 x 2048 to 5632 x 5632 at k = 4096 and 512 and to 65536 x 256 x 256; a round that is not full takes less than a full one.  (bf16,
     // large / small: 4096 x 4096 x 4096 62 / 74, 2560 x 3584 x 4096 45 / 55, 5632 x 5632 x 4096 105 / 135, 2048 x 2048 x 4096 61 / 26,
     // 4096 x 4096 x 512 19.5 / 17.2.)  Large tiles ask for blocks two ahead, so that they need two.
     const double r = (double)tiles(256) / UNITS, q = (double)small / (2 * UNITS);

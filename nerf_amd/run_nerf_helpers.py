@@ -123,8 +123,8 @@ class NeRF(nn.Module):
     (ops.linear) -- same results, autograd included (inputs too), none of the fusion.
 
     Two options that upstream lacks, for wide and deep networks, take the same layer-by-layer route: layer_norm=True puts
-    a layer norm (ops.layer_norm) behind the ReLU of every pts_linears layer, and layer_dtype = 'fp8' runs the W-wide products in
-    8 bits (ops.linear_fp8)."""
+    a layer norm (ops.layer_norm) behind the ReLU of every pts_linears layer, and layer_dtype = 'fp8' runs the W-wide products on
+    operands held in 8 bits (ops.linear_fp8).  At the fused shape they cost its kernels: a training step of 1024 rays 4.5 -> 20.8 and 8.3 ms."""
 
     def __init__(self, D=8, W=256, input_ch=3, input_ch_views=3, output_ch=4, skips=[4], use_viewdirs=False,
                  layer_norm=False):

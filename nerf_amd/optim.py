@@ -301,7 +301,8 @@ class AdamW(torch.optim.Optimizer):
     Parameters are fp32, bf16 or fp16 and contiguous, on a HIP device when the step is taken.  `state[p]` holds ordinary tensors:
       step         fp32 scalar on the device
       exp_avg, exp_avg_sq   state_bits = 32: fp32, as torch.optim.AdamW's (whose checkpoints of fp32 parameters load, and the reverse);
-                   state_bits = 8: float8_e4m3fn and float8_e5m2, relative to `scale`
+                   state_bits = 8: float8_e4m3fn and float8_e5m2, relative to `scale` (for this class alone: torch's would take the
+                   codes for moments)
       scale        state_bits = 8: fp32 [blocks of 128 consecutive elements, 2]: the largest |exp_avg| / 448 and exp_avg_sq / 57344, at
                    least 1e-38 unless all are 0
       master       16-bit parameters: the fp32 values they are rounded from (an element of the parameter that was written from
